@@ -155,6 +155,92 @@ int wsp_hip_attention_static(const float* q, int q_count, const float* keys, con
                              int k_count, int width, int heads, int causal, float scale, float* out,
                              void* stream, char* error, int error_capacity);
 
+/* ---- a paged cache ---------------------------------------------------------
+ * No reference counterpart: the reference's caches are one run of rows for one
+ * sequence (Decoder/Decoder.cpp:194-227). Here keys and values lie in pages of
+ * page_rows positions out of one pool, a sequence owns the pages its row of a
+ * table names, sequences have lengths of their own, and the rows may be held in
+ * 16 or 8 bits. wsp_hip_paged_append writes new rows, wsp_hip_paged_read reads
+ * rows back, wsp_hip_paged_attention is wsp_hip_attention over the pages. All
+ * three are ordered on the context's stream and run on its device whatever the
+ * current one is, allocate nothing and clear nothing, so they can be captured
+ * into a HIP graph (the table, lengths and starts are read when it is replayed).
+ * The attention's partial rows go through the context's scratch, so calls on one
+ * context, and replays of graphs captured from it, have to be ordered. */
+
+/* WSP_E4M3, a storage of paged caches only: 8-bit floating point (4 exponent
+ * and 3 fraction bits, largest 448, no infinities) with one power of two 2^k
+ * for each row (one position of one head), k held in a byte as k + 127. k is
+ * the least in [-80, 120] that brings the row's largest finite magnitude to 448
+ * or below, so the division is exact and the rounding to 8 bits (to nearest,
+ * ties to even) the only one; magnitudes below 2^-90 become zero, infinities
+ * and NaN become NaN. F16 and BF16 rows are rounded to nearest, F32 kept. */
+enum
+{
+    WSP_E4M3 = 3
+};
+
+/* A pool of pages; everything but the struct itself is device memory of the
+ * context's device, pools at 16 bytes. Slots that no sequence has written may
+ * hold anything. */
+typedef struct wsp_paged_cache
+{
+    int storage;    /* WSP_F32, WSP_F16, WSP_BF16 or WSP_E4M3 */
+    int pages;      /* pages in the pool */
+    int page_rows;  /* positions a page holds: a power of two, 16 to 1024 */
+    int heads;      /* key and value heads */
+    int head_width; /* a multiple of 16, at most 128 */
+    void* keys;     /* [pages][heads][page_rows][head_width] */
+    void* values;   /* the same */
+    uint8_t* key_exponents;   /* [pages][heads][page_rows], E4M3 only */
+    uint8_t* value_exponents; /* the same */
+} wsp_paged_cache;
+
+/* The new rows of a call and the sequences they belong to. Packed rows
+ * starts[s] .. starts[s + 1] - 1 are sequence s's last positions: with n of
+ * them, packed row starts[s] + i is position lengths[s] - n + i. starts
+ * ascends; rows past starts[sequences] belong to nobody and are neither read nor
+ * written, and a sequence may have none. A row before its sequence's start
+ * (n > lengths[s]) is none: it is not stored, reads back as zeros and sees no
+ * key. No two rows of an append may share a slot. Position p lies in the page
+ * pages[s·table_width + p / page_rows]; a page that is not in the pool, or
+ * a position past the table, is never touched: append drops the row, read gives
+ * NaN, and attention gives NaN for the rows that see such a key. Entries past a
+ * sequence's length are not read. */
+typedef struct wsp_paged_rows
+{
+    int sequences;
+    int rows;            /* rows the packed tensors hold, at least starts[sequences] */
+    int max_count;       /* attention: no sequence has more new rows (more are left as they were) */
+    int max_length;      /* attention: no length is larger (else that sequence's rows are NaN) */
+    int table_width;     /* pages a row of the table names */
+    const int* starts;   /* device [sequences + 1] */
+    const int* lengths;  /* device [sequences], the new rows among them */
+    const int* pages;    /* device [sequences][table_width] */
+} wsp_paged_rows;
+
+/* Stores the new rows: keys and values are f32 [rows][heads·head_width], rows
+ * key_stride and value_stride floats apart (columns of a wider tensor, such as a
+ * fused projection's output; they may start at any float). */
+int wsp_hip_paged_append(wsp_hip_ctx* ctx, const wsp_paged_cache* cache, const wsp_paged_rows* rows,
+                         const float* keys, int key_stride, const float* values, int value_stride);
+
+/* The rows' stored values widened to f32 (exact), laid out as append takes
+ * them. With counts equal to the lengths it reads whole sequences. */
+int wsp_hip_paged_read(wsp_hip_ctx* ctx, const wsp_paged_cache* cache, const wsp_paged_rows* rows, float* keys,
+                       int key_stride, float* values, int value_stride);
+
+/* Attention of the packed rows q (f32 [rows][heads·head_width], rows q_stride
+ * floats apart) over their sequences' pages, into out (rows out_stride floats
+ * apart, no overlap with q): causal rows see the positions up to their own,
+ * others every position before lengths[s]. heads is a multiple of the cache's
+ * heads; query head h reads cache head h / (heads / cache heads). scale
+ * multiplies the summed dot product. A row that sees no key gets zeros; keys and
+ * values that a row does not see do not reach it, whatever they hold. */
+int wsp_hip_paged_attention(wsp_hip_ctx* ctx, const wsp_paged_cache* cache, const wsp_paged_rows* rows,
+                            const float* q, int q_stride, int heads, int causal, float scale, float* out,
+                            int out_stride);
+
 /* out[r] = the first j maximising logits[r * row_length + j] over the j with
  * mask[j] == 0 (mask may be null); all suppressed gives 0. Replaces Argmax
  * (Kernels/Argmax.h:46-262, Kernels/Argmax.cpp:43-81). */

@@ -29,6 +29,7 @@ WSP_ERR_LOGIC = -5
 WSP_ERR_DEVICE = -6
 
 WSP_F32, WSP_F16, WSP_BF16 = 0, 1, 2
+WSP_E4M3 = 3  # paged caches only
 WSP_LINEAR_GELU, WSP_LINEAR_RESIDUAL = 1, 2
 
 WSP_KIND_NONE, WSP_KIND_MODEL_ERROR, WSP_KIND_LOGIC_ERROR, WSP_KIND_INVALID_ARGUMENT, WSP_KIND_RUNTIME_ERROR = range(5)
@@ -82,6 +83,16 @@ class wsp_mel_shape(ctypes.Structure):
     _fields_ = [(n, c_int) for n in ("sample_count", "fft_length", "hop_length", "frame_count", "mel_count")]
 
 
+class wsp_paged_cache(ctypes.Structure):
+    _fields_ = [(n, c_int) for n in ("storage", "pages", "page_rows", "heads", "head_width")] + [
+        (n, c_void_p) for n in ("keys", "values", "key_exponents", "value_exponents")]
+
+
+class wsp_paged_rows(ctypes.Structure):
+    _fields_ = [(n, c_int) for n in ("sequences", "rows", "max_count", "max_length", "table_width")] + [
+        (n, c_void_p) for n in ("starts", "lengths", "pages")]
+
+
 class wsp_special_tokens(ctypes.Structure):
     _fields_ = [(name, c_int) for name in ("end_of_text", "start_of_transcript", "start_of_previous",
                                            "start_of_language_model", "translate", "transcribe", "no_timestamps",
@@ -103,6 +114,12 @@ SIGNATURES = {
                                   c_float, c_void_p]),
     "wsp_hip_attention_static": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float,
                                          c_void_p, c_void_p, ctypes.c_char_p, c_int]),
+    "wsp_hip_paged_append": (c_int, [c_void_p, ctypes.POINTER(wsp_paged_cache), ctypes.POINTER(wsp_paged_rows),
+                                     c_void_p, c_int, c_void_p, c_int]),
+    "wsp_hip_paged_read": (c_int, [c_void_p, ctypes.POINTER(wsp_paged_cache), ctypes.POINTER(wsp_paged_rows),
+                                   c_void_p, c_int, c_void_p, c_int]),
+    "wsp_hip_paged_attention": (c_int, [c_void_p, ctypes.POINTER(wsp_paged_cache), ctypes.POINTER(wsp_paged_rows),
+                                        c_void_p, c_int, c_int, c_int, c_float, c_void_p, c_int]),
     "wsp_hip_argmax": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p]),
     "wsp_hip_project_cross_kv": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int,
                                          c_void_p, c_void_p]),
