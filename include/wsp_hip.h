@@ -236,7 +236,8 @@ int wsp_hip_paged_read(wsp_hip_ctx* ctx, const wsp_paged_cache* cache, const wsp
  * others every position before lengths[s]. heads is a multiple of the cache's
  * heads; query head h reads cache head h / (heads / cache heads). scale
  * multiplies the summed dot product. A row that sees no key gets zeros; keys and
- * values that a row does not see do not reach it, whatever they hold. */
+ * values that a row does not see do not reach it, whatever they hold. (One that
+ * sees an infinity or NaN in a key is NaN, in F32 storage as fp32 has it.) */
 int wsp_hip_paged_attention(wsp_hip_ctx* ctx, const wsp_paged_cache* cache, const wsp_paged_rows* rows,
                             const float* q, int q_stride, int heads, int causal, float scale, float* out,
                             int out_stride);

@@ -161,6 +161,26 @@ def test_batch_split_sizing_and_refusals_on_the_host():
     assert "FAIL" not in result.stdout and result.stdout.count("ok ") == 32, result.stdout
 
 
+def test_paged_refusals_and_lookups_on_the_host():
+    # The paged cache's refusals and the look-ups its kernels take every address
+    # from are host code too (csrc/paged_plan.h), checked here on the CPU under
+    # ASan/UBSan: bad tables, lengths and starts never lead outside.
+    import subprocess
+    path = os.path.join(ROOT, "tests", "native", "_build", "paged_plan_check")
+    subprocess.run(["make", "-s", "_build/paged_plan_check"], cwd=os.path.join(ROOT, "tests", "native"), check=True)
+    result = subprocess.run([path], capture_output=True, text=True, timeout=60)
+    assert result.returncode == 0, result.stdout + result.stderr
+    assert "FAIL" not in result.stdout and result.stdout.count("ok ") >= 33, result.stdout
+
+
+def test_paged_calls_refuse_without_a_context():
+    from whispereacp_amd import _native as N
+    lib = ensure_library()
+    assert lib.wsp_hip_paged_append(None, None, None, None, 0, None, 0) == N.WSP_ERR_ARGUMENT
+    assert lib.wsp_hip_paged_read(None, None, None, None, 0, None, 0) == N.WSP_ERR_ARGUMENT
+    assert lib.wsp_hip_paged_attention(None, None, None, None, 0, 1, 1, 1.0, None, 0) == N.WSP_ERR_ARGUMENT
+
+
 def test_every_gpu_is_prepared_once():
     # The products' kernels ask for more LDS than a launch gets unasked, on each
     # GPU a process uses; the once-per-device guard is host code

@@ -1,0 +1,399 @@
+// The paged cache's kernels: storing new rows, reading rows back, and attention
+// over pages (include/wsp_hip.h, wsp_hip_paged_*). Every address of the pool
+// comes from paged_plan.h's checked lookups.
+#include "device_common.h"
+#include "paged.h"
+#include "paged_plan.h"
+
+#include <cmath>
+
+namespace wsp::paged
+{
+namespace
+{
+constexpr int kBlock = 256;
+constexpr int kE4M3 = WSP_E4M3;
+constexpr int kMinExponent = -80, kMaxExponent = 120, kExponentBias = 127;
+
+// The power of two of an E4M3 row: the least k in range with amax <= 448·2^k
+// (448 = 1.75·2^8).
+__device__ __forceinline__ int row_exponent(float amax)
+{
+    const uint32_t bits = __float_as_uint(amax);
+    const int k = (int) (bits >> 23) - 127 - 8 + ((bits & 0x7FFFFFu) > 0x600000u);
+    return min(max(k, kMinExponent), kMaxExponent);
+}
+
+__device__ __forceinline__ float finite_magnitude(float v)
+{
+    const float a = fabsf(v);
+    return a < INFINITY ? a : 0.f; // (false for NaN too)
+}
+
+// Four values as E4M3 bytes of v·2^-k; infinities and NaN become NaN.
+__device__ __forceinline__ uint32_t to_e4m3(const float4v v, int k)
+{
+    float s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        s[i] = isfinite(v[i]) ? ldexpf(v[i], -k) : __builtin_nanf("");
+    int packed = __builtin_amdgcn_cvt_pk_fp8_f32(s[0], s[1], 0, false);
+    packed = __builtin_amdgcn_cvt_pk_fp8_f32(s[2], s[3], packed, true);
+    return (uint32_t) packed;
+}
+
+__device__ __forceinline__ float4v from_e4m3(uint32_t packed)
+{
+    const auto low = __builtin_amdgcn_cvt_pk_f32_fp8((int) packed, false);
+    const auto high = __builtin_amdgcn_cvt_pk_f32_fp8((int) packed, true);
+    return float4v {low[0], low[1], high[0], high[1]};
+}
+
+// Four consecutive stored values, `index` a multiple of four; E4M3 without its
+// row's power of two.
+template <int ST>
+__device__ __forceinline__ float4v load_stored4(const void* pool, size_t index)
+{
+    if constexpr (ST == kF32)
+        return *reinterpret_cast<const float4v*>(static_cast<const float*>(pool) + index);
+    else if constexpr (ST == kF16)
+    {
+        const half4 h = *reinterpret_cast<const half4*>(static_cast<const _Float16*>(pool) + index);
+        return float4v {(float) h[0], (float) h[1], (float) h[2], (float) h[3]};
+    }
+    else if constexpr (ST == kBF16)
+    {
+        const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(pool) + index);
+        return float4v {__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16),
+                        __uint_as_float(u.y & 0xFFFF0000u)};
+    }
+    else
+        return from_e4m3(*reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(pool) + index));
+}
+
+template <int ST>
+__device__ __forceinline__ void store_stored4(void* pool, size_t index, const float4v v, int k)
+{
+    if constexpr (ST == kF32)
+        *reinterpret_cast<float4v*>(static_cast<float*>(pool) + index) = v;
+    else if constexpr (ST == kF16)
+    {
+        const half4 h = {(_Float16) v[0], (_Float16) v[1], (_Float16) v[2], (_Float16) v[3]};
+        *reinterpret_cast<half4*>(static_cast<_Float16*>(pool) + index) = h;
+    }
+    else if constexpr (ST == kBF16)
+    {
+        typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+        const bf16x4 h = {(__bf16) v[0], (__bf16) v[1], (__bf16) v[2], (__bf16) v[3]};
+        *reinterpret_cast<bf16x4*>(static_cast<uint16_t*>(pool) + index) = h;
+    }
+    else
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(pool) + index) = to_e4m3(v, k);
+}
+
+// What the kernels take of a cache and its rows.
+struct Cache
+{
+    int pages, page_shift, heads, head_width;
+    void* keys;
+    void* values;
+    uint8_t* key_exponents;
+    uint8_t* value_exponents;
+};
+struct Rows
+{
+    int sequences, rows, max_count, max_length, table_width;
+    const int* starts;
+    const int* lengths;
+    const int* pages;
+};
+
+__device__ __forceinline__ int page_at(const Cache& cache, const Rows& rows, int sequence, int position)
+{
+    return page_of(rows.pages + (size_t) sequence * rows.table_width, rows.table_width, cache.page_shift, cache.pages,
+                   position);
+}
+
+// ---------------------------------------------------------------------------
+// Append and read: LANES lanes (16 for heads up to 64 wide, 32 for wider ones)
+// a (row, head), four values of its key and of its value each. Append takes the
+// row's largest magnitude over those lanes, so a row is read once.
+// ---------------------------------------------------------------------------
+template <int LANES>
+__device__ __forceinline__ float lanes_max(float v)
+{
+#pragma unroll
+    for (int offset = LANES / 2; offset > 0; offset >>= 1)
+        v = fmaxf(v, __shfl_xor(v, offset, LANES));
+    return v;
+}
+
+template <int ST, int LANES>
+__global__ void __launch_bounds__(kBlock) append_kernel(Cache cache, Rows rows, const float* __restrict__ keys,
+                                                        int key_stride, const float* __restrict__ values,
+                                                        int value_stride)
+{
+    const long long unit = ((long long) blockIdx.x * kBlock + threadIdx.x) / LANES;
+    const int row = (int) (unit / cache.heads), head = (int) (unit % cache.heads);
+    const int c = 4 * (threadIdx.x % LANES);
+    if (row >= rows.rows) // (whole groups of lanes leave together)
+        return;
+    const int sequence = sequence_of(rows.starts, rows.sequences, row);
+    if (sequence < 0)
+        return;
+    const long long position = position_of(rows.starts, rows.lengths, sequence, row);
+    const int page = position < 0 ? -1 : page_at(cache, rows, sequence, (int) position);
+    if (page < 0)
+        return;
+    const bool inside = c < cache.head_width;
+    float4v k = {0.f, 0.f, 0.f, 0.f}, v = k;
+    if (inside)
+    {
+        k = *reinterpret_cast<const float4u*>(keys + (size_t) row * key_stride + (size_t) head * cache.head_width + c);
+        v = *reinterpret_cast<const float4u*>(values + (size_t) row * value_stride + (size_t) head * cache.head_width
+                                              + c);
+    }
+    const size_t slot = pool_row(page, head, (int) position & ((1 << cache.page_shift) - 1), cache.heads,
+                                 cache.page_shift);
+    int key_exponent = 0, value_exponent = 0;
+    if constexpr (ST == kE4M3)
+    {
+        float key_max = 0.f, value_max = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+        {
+            key_max = fmaxf(key_max, finite_magnitude(k[i]));
+            value_max = fmaxf(value_max, finite_magnitude(v[i]));
+        }
+        key_exponent = row_exponent(lanes_max<LANES>(key_max));
+        value_exponent = row_exponent(lanes_max<LANES>(value_max));
+        if (c == 0)
+        {
+            cache.key_exponents[slot] = (uint8_t) (key_exponent + kExponentBias);
+            cache.value_exponents[slot] = (uint8_t) (value_exponent + kExponentBias);
+        }
+    }
+    if (inside)
+    {
+        store_stored4<ST>(cache.keys, slot * cache.head_width + c, k, key_exponent);
+        store_stored4<ST>(cache.values, slot * cache.head_width + c, v, value_exponent);
+    }
+}
+
+template <int ST, int LANES>
+__global__ void __launch_bounds__(kBlock) read_kernel(Cache cache, Rows rows, float* __restrict__ keys,
+                                                      int key_stride, float* __restrict__ values, int value_stride)
+{
+    const long long unit = ((long long) blockIdx.x * kBlock + threadIdx.x) / LANES;
+    const int row = (int) (unit / cache.heads), head = (int) (unit % cache.heads);
+    const int c = 4 * (threadIdx.x % LANES);
+    if (row >= rows.rows || c >= cache.head_width)
+        return;
+    const int sequence = sequence_of(rows.starts, rows.sequences, row);
+    if (sequence < 0)
+        return;
+    const long long position = position_of(rows.starts, rows.lengths, sequence, row);
+    float4v k = {0.f, 0.f, 0.f, 0.f}, v = k;
+    if (position >= 0)
+    {
+        const int page = page_at(cache, rows, sequence, (int) position);
+        if (page < 0)
+            k = v = float4v {0.f, 0.f, 0.f, 0.f} + __builtin_nanf("");
+        else
+        {
+            const size_t slot = pool_row(page, head, (int) position & ((1 << cache.page_shift) - 1), cache.heads,
+                                         cache.page_shift);
+            k = load_stored4<ST>(cache.keys, slot * cache.head_width + c);
+            v = load_stored4<ST>(cache.values, slot * cache.head_width + c);
+            if constexpr (ST == kE4M3)
+            {
+                const int key_exponent = (int) cache.key_exponents[slot] - kExponentBias;
+                const int value_exponent = (int) cache.value_exponents[slot] - kExponentBias;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                {
+                    k[i] = ldexpf(k[i], key_exponent);
+                    v[i] = ldexpf(v[i], value_exponent);
+                }
+            }
+        }
+    }
+    *reinterpret_cast<float4u*>(keys + (size_t) row * key_stride + (size_t) head * cache.head_width + c) = k;
+    *reinterpret_cast<float4u*>(values + (size_t) row * value_stride + (size_t) head * cache.head_width + c) = v;
+}
+
+// ---------------------------------------------------------------------------
+// Attention: a block for each (packed row, query head), 16 groups of 16 lanes,
+// each with every sixteenth key it sees: eight channels a lane, an online
+// softmax (the running maximum and sum, the row rescaled when the maximum
+// grows) a group, and the groups merged through LDS.
+// ---------------------------------------------------------------------------
+template <int ST>
+__global__ void __launch_bounds__(kBlock) row_attention_kernel(Cache cache, Rows rows, const float* __restrict__ q,
+                                                               int q_stride, int heads, int causal, float scale,
+                                                               float* __restrict__ out, int out_stride)
+{
+    constexpr int kGroups = kBlock / 16;
+    __shared__ float tops[kGroups], totals[kGroups];
+    __shared__ float sums[kGroups][kMaxHeadWidth];
+
+    const int row = blockIdx.x / heads, head = blockIdx.x % heads;
+    const int cached = head / (heads / cache.heads), width = cache.head_width;
+    const int sequence = sequence_of(rows.starts, rows.sequences, row);
+    if (sequence < 0 || row - rows.starts[sequence] >= rows.max_count)
+        return;
+    const int length = rows.lengths[sequence];
+    const long long position = position_of(rows.starts, rows.lengths, sequence, row);
+    const int seen = position < 0 ? 0 : causal ? (int) position + 1 : length;
+
+    const int group = threadIdx.x / 16, c = 8 * (threadIdx.x % 16);
+    const bool inside = c < width;
+    const float4v none = {0.f, 0.f, 0.f, 0.f};
+    float4v q0 = none, q1 = none, o0 = none, o1 = none;
+    if (inside)
+    {
+        const float* at = q + (size_t) row * q_stride + (size_t) head * width + c;
+        q0 = *reinterpret_cast<const float4u*>(at);
+        q1 = *reinterpret_cast<const float4u*>(at + 4);
+    }
+    float m = -INFINITY, l = 0.f;
+    if (length > rows.max_length)
+        l = __builtin_nanf("");
+    else
+        for (int j = group; j < seen; j += kGroups)
+        {
+            const int page = page_at(cache, rows, sequence, j);
+            if (page < 0)
+            {
+                l = __builtin_nanf("");
+                break;
+            }
+            const size_t slot = pool_row(page, cached, j & ((1 << cache.page_shift) - 1), cache.heads,
+                                         cache.page_shift);
+            float4v k0 = none, k1 = none, v0 = none, v1 = none;
+            if (inside)
+            {
+                k0 = load_stored4<ST>(cache.keys, slot * width + c);
+                k1 = load_stored4<ST>(cache.keys, slot * width + c + 4);
+                v0 = load_stored4<ST>(cache.values, slot * width + c);
+                v1 = load_stored4<ST>(cache.values, slot * width + c + 4);
+            }
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                s += q0[i] * k0[i] + q1[i] * k1[i];
+            s = sum16(s) * scale;
+            if (s == -INFINITY)
+                continue; // (weight zero; against a maximum of -inf it would be NaN)
+            float gain = 1.f;
+            if constexpr (ST == kE4M3)
+            {
+                s = ldexpf(s, (int) cache.key_exponents[slot] - kExponentBias);
+                gain = ldexpf(1.f, (int) cache.value_exponents[slot] - kExponentBias);
+            }
+            const float top = fmaxf(m, s);
+            const float rescale = expf(m - top), p = expf(s - top);
+            l = l * rescale + p;
+            o0 = o0 * rescale + v0 * (p * gain);
+            o1 = o1 * rescale + v1 * (p * gain);
+            m = top;
+        }
+    if (threadIdx.x % 16 == 0)
+    {
+        tops[group] = m;
+        totals[group] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+        sums[group][c + i] = o0[i];
+        sums[group][c + 4 + i] = o1[i];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < width; i += kBlock)
+    {
+        float largest = -INFINITY;
+        for (int w = 0; w < kGroups; ++w)
+            largest = fmaxf(largest, tops[w]);
+        float numerator = 0.f, denominator = 0.f;
+        for (int w = 0; w < kGroups; ++w)
+            if (totals[w] != 0.f) // (a group without a key)
+            {
+                const float factor = expf(tops[w] - largest);
+                numerator += factor * sums[w][i];
+                denominator += factor * totals[w];
+            }
+        out[(size_t) row * out_stride + (size_t) head * width + i] = denominator == 0.f ? 0.f : numerator / denominator;
+    }
+}
+
+Cache device_cache(const wsp_paged_cache& c)
+{
+    return {c.pages, shift_of(c.page_rows), c.heads, c.head_width, c.keys, c.values, c.key_exponents, c.value_exponents};
+}
+
+Rows device_rows(const wsp_paged_rows& r)
+{
+    return {r.sequences, r.rows, r.max_count, r.max_length, r.table_width, r.starts, r.lengths, r.pages};
+}
+
+// f called with the storage as a compile-time constant.
+template <class F>
+void by_storage(int storage, F&& f)
+{
+    switch (storage)
+    {
+        case WSP_F32: return f(std::integral_constant<int, kF32> {});
+        case WSP_F16: return f(std::integral_constant<int, kF16> {});
+        case WSP_BF16: return f(std::integral_constant<int, kBF16> {});
+        default: return f(std::integral_constant<int, kE4M3> {});
+    }
+}
+
+// The same with the storage and the lanes of a (row, head).
+template <class F>
+void by_lanes(const wsp_paged_cache& cache, F&& f)
+{
+    by_storage(cache.storage, [&](auto storage) {
+        cache.head_width <= 64 ? f(storage, std::integral_constant<int, 16> {})
+                               : f(storage, std::integral_constant<int, 32> {});
+    });
+}
+
+unsigned row_blocks(const wsp_paged_cache& cache, const wsp_paged_rows& rows)
+{
+    const long long threads = (long long) rows.rows * cache.heads * (cache.head_width <= 64 ? 16 : 32);
+    return (unsigned) ((threads + kBlock - 1) / kBlock);
+}
+} // namespace
+
+hipError_t append(hipStream_t stream, const wsp_paged_cache& cache, const wsp_paged_rows& rows, const float* keys,
+                  int key_stride, const float* values, int value_stride)
+{
+    by_lanes(cache, [&](auto storage, auto lanes) {
+        append_kernel<storage(), lanes()><<<row_blocks(cache, rows), kBlock, 0, stream>>>(
+            device_cache(cache), device_rows(rows), keys, key_stride, values, value_stride);
+    });
+    return hipGetLastError();
+}
+
+hipError_t read(hipStream_t stream, const wsp_paged_cache& cache, const wsp_paged_rows& rows, float* keys,
+                int key_stride, float* values, int value_stride)
+{
+    by_lanes(cache, [&](auto storage, auto lanes) {
+        read_kernel<storage(), lanes()><<<row_blocks(cache, rows), kBlock, 0, stream>>>(
+            device_cache(cache), device_rows(rows), keys, key_stride, values, value_stride);
+    });
+    return hipGetLastError();
+}
+
+hipError_t attention(hipStream_t stream, const wsp_paged_cache& cache, const wsp_paged_rows& rows, const float* q,
+                     int q_stride, int heads, bool causal, float scale, float* out, int out_stride)
+{
+    by_storage(cache.storage, [&](auto storage) {
+        row_attention_kernel<storage()><<<(unsigned) (rows.rows * heads), kBlock, 0, stream>>>(
+            device_cache(cache), device_rows(rows), q, q_stride, heads, causal, scale, out, out_stride);
+    });
+    return hipGetLastError();
+}
+} // namespace wsp::paged

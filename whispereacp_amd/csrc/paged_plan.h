@@ -1,0 +1,128 @@
+// The paged cache's arithmetic that needs no device: what the entry points
+// refuse, where a position lies, and which packed row is whose. The kernels take
+// every address from here (constexpr functions are both host and device code),
+// so a bad table, length or start never leads outside the pool.
+#pragma once
+
+#include "../../include/wsp_hip.h"
+
+#include <cstdarg>
+#include <cstddef>
+#include <cstdint>
+#include <cstdio>
+
+namespace wsp::paged
+{
+constexpr int kMaxHeadWidth = 128;
+constexpr int kMinPageRows = 16, kMaxPageRows = 1024;
+
+// The page of `position` in a sequence's row of the table, or -1: a position
+// before the sequence or past the table, or a page that is not in the pool.
+constexpr int page_of(const int* table, int table_width, int page_shift, int pages, int position)
+{
+    const int block = position >> page_shift;
+    if (position < 0 || block >= table_width)
+        return -1;
+    const int page = table[block];
+    return page >= 0 && page < pages ? page : -1;
+}
+
+// The pool's row of a head at a place in a page (rows of head_width values).
+constexpr size_t pool_row(int page, int head, int place, int heads, int page_shift)
+{
+    return ((((size_t) page * heads + head) << page_shift) + place);
+}
+
+// The sequence of packed row `row`, or -1. The guess (row r is sequence r's, as
+// in a step of one token each) saves such a step the search.
+constexpr int sequence_of(const int* starts, int sequences, int row)
+{
+    if (row < sequences && starts[row] == row && starts[row + 1] == row + 1)
+        return row;
+    int first = 0, last = sequences; // starts[i] <= row for i < first, > row for i >= last
+    while (first < last)
+    {
+        const int middle = first + (last - first) / 2;
+        if (starts[middle] <= row)
+            first = middle + 1;
+        else
+            last = middle;
+    }
+    const int sequence = first - 1;
+    return sequence >= 0 && row < starts[sequence + 1] ? sequence : -1;
+}
+
+// Packed row `row`'s position (before 0: none), given its sequence.
+constexpr long long position_of(const int* starts, const int* lengths, int sequence, int row)
+{
+    return (long long) lengths[sequence] - ((long long) starts[sequence + 1] - row);
+}
+
+constexpr int shift_of(int page_rows)
+{
+    int shift = 0;
+    while ((1 << shift) < page_rows)
+        ++shift;
+    return shift;
+}
+
+constexpr size_t storage_bytes(int storage)
+{
+    return storage == WSP_F32 ? 4 : storage == WSP_E4M3 ? 1 : 2;
+}
+
+inline int say(char* why, size_t size, int code, const char* format, ...)
+{
+    va_list args;
+    va_start(args, format);
+    std::vsnprintf(why, size, format, args);
+    va_end(args);
+    return code;
+}
+
+// Why a call over this cache and these rows is refused: WSP_OK, or a status
+// with the reason in `why`.
+inline int refusal(const wsp_paged_cache* cache, const wsp_paged_rows* rows, char* why, size_t size)
+{
+    if (cache == nullptr || rows == nullptr)
+        return say(why, size, WSP_ERR_ARGUMENT, "paged: null cache or rows");
+    if (cache->storage != WSP_F32 && cache->storage != WSP_F16 && cache->storage != WSP_BF16
+        && cache->storage != WSP_E4M3)
+        return say(why, size, WSP_ERR_ARGUMENT, "paged: unknown storage %d", cache->storage);
+    if (cache->pages <= 0 || cache->heads <= 0)
+        return say(why, size, WSP_ERR_ARGUMENT, "paged: %d pages of %d heads", cache->pages, cache->heads);
+    if (cache->head_width <= 0 || cache->head_width % 16 != 0 || cache->head_width > kMaxHeadWidth)
+        return say(why, size, WSP_ERR_LOGIC, "paged: heads up to %d wide in multiples of 16, and not %d", kMaxHeadWidth,
+                   cache->head_width);
+    if (cache->page_rows < kMinPageRows || cache->page_rows > kMaxPageRows
+        || (cache->page_rows & (cache->page_rows - 1)) != 0)
+        return say(why, size, WSP_ERR_LOGIC, "paged: pages hold a power of two of %d to %d positions, and not %d", kMinPageRows,
+                   kMaxPageRows, cache->page_rows);
+    if (cache->keys == nullptr || cache->values == nullptr)
+        return say(why, size, WSP_ERR_ARGUMENT, "paged: null pool");
+    if (reinterpret_cast<uintptr_t>(cache->keys) % 16 != 0 || reinterpret_cast<uintptr_t>(cache->values) % 16 != 0)
+        return say(why, size, WSP_ERR_ARGUMENT, "paged: pools lie at 16 bytes");
+    if (cache->storage == WSP_E4M3 && (cache->key_exponents == nullptr || cache->value_exponents == nullptr))
+        return say(why, size, WSP_ERR_ARGUMENT, "paged: E4M3 without exponents");
+    if (rows->sequences < 0 || rows->rows < 0 || rows->max_count < 0 || rows->max_length < 0 || rows->table_width < 0)
+        return say(why, size, WSP_ERR_ARGUMENT, "paged: %d sequences, %d rows, at most %d of %d, %d pages a sequence",
+                   rows->sequences, rows->rows, rows->max_count, rows->max_length, rows->table_width);
+    if (rows->sequences > 0 && (rows->starts == nullptr || rows->lengths == nullptr))
+        return say(why, size, WSP_ERR_ARGUMENT, "paged: null starts or lengths");
+    if (rows->sequences > 0 && rows->table_width > 0 && rows->pages == nullptr)
+        return say(why, size, WSP_ERR_ARGUMENT, "paged: null table");
+    return WSP_OK;
+}
+
+// The same for packed tensors of `heads` heads, rows `stride` floats apart.
+inline int refusal_of_tensor(const wsp_paged_cache* cache, const wsp_paged_rows* rows, const char* name,
+                             const void* data, int heads, int stride, char* why, size_t size)
+{
+    if (data == nullptr && rows->rows > 0)
+        return say(why, size, WSP_ERR_ARGUMENT, "paged: null %s", name);
+    if (stride < (long long) heads * cache->head_width)
+        return say(why, size, WSP_ERR_SHAPE, "paged: %s rows of %d heads of %d lie %d floats apart", name, heads,
+                   cache->head_width, stride);
+    return WSP_OK;
+}
+} // namespace wsp::paged

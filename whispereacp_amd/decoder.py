@@ -63,6 +63,7 @@ class KernelContext:
     def __init__(self, shape: DecoderShape, device: int = 0):
         self.lib = N.load()
         self.shape = shape
+        self.device = device
         handle = ctypes.c_void_p()
         self._cshape = c_shape(shape)
         status = self.lib.wsp_hip_ctx_create(ctypes.byref(self._cshape), device, current_stream(),
@@ -98,6 +99,35 @@ class KernelContext:
     def attention(self, q, q_count, keys, values, k_count, width, heads, causal, scale, out):
         self._check(self.lib.wsp_hip_attention(self.handle, ptr(q), q_count, ptr(keys), ptr(values), k_count,
                                                width, heads, int(causal), scale, ptr(out)))
+
+    def paged_append(self, cache, rows, keys, values):
+        """Stores the packed rows keys and values [rows.rows, heads·head_width] in
+        their sequences' pages (paged.PagedCache, paged.PagedRows)."""
+        cache.check(self.device)
+        rows.check(self.device)
+        width = cache.heads * cache.head_width
+        self._check(self.lib.wsp_hip_paged_append(
+            self.handle, cache.table, rows.table, ptr(keys), rows.stride(keys, width, self.device), ptr(values),
+            rows.stride(values, width, self.device)))
+
+    def paged_read(self, cache, rows, keys, values):
+        """Writes the packed rows' stored values to keys and values, fp32."""
+        cache.check(self.device)
+        rows.check(self.device)
+        width = cache.heads * cache.head_width
+        self._check(self.lib.wsp_hip_paged_read(
+            self.handle, cache.table, rows.table, ptr(keys), rows.stride(keys, width, self.device), ptr(values),
+            rows.stride(values, width, self.device)))
+
+    def paged_attention(self, cache, rows, q, heads, causal, scale, out):
+        """Attention of the packed rows q [rows.rows, heads·head_width] over their
+        sequences' pages, into out."""
+        cache.check(self.device)
+        rows.check(self.device)
+        width = heads * cache.head_width
+        self._check(self.lib.wsp_hip_paged_attention(
+            self.handle, cache.table, rows.table, ptr(q), rows.stride(q, width, self.device), heads, int(causal), scale,
+            ptr(out), rows.stride(out, width, self.device)))
 
     def argmax(self, logits, rows, row_length, mask, out):
         self._check(self.lib.wsp_hip_argmax(self.handle, ptr(logits), rows, row_length, ptr(mask), ptr(out)))
