@@ -1,5 +1,5 @@
-// Host-side launchers of the paged cache's kernels (paged.hip); arguments are
-// checked by paged_capi.hip.
+// Host-side launchers of the paged cache's kernels (paged.hip,
+// paged_attention.hip); arguments are checked by paged_capi.hip.
 #pragma once
 
 #include "../../include/wsp_hip.h"
@@ -13,5 +13,6 @@ hipError_t append(hipStream_t stream, const wsp_paged_cache& cache, const wsp_pa
 hipError_t read(hipStream_t stream, const wsp_paged_cache& cache, const wsp_paged_rows& rows, float* keys,
                 int key_stride, float* values, int value_stride);
 hipError_t attention(hipStream_t stream, const wsp_paged_cache& cache, const wsp_paged_rows& rows, const float* q,
-                     int q_stride, int heads, bool causal, float scale, float* out, int out_stride);
+                     int q_stride, int heads, bool causal, float scale, float* out, int out_stride,
+                     void* scratch, size_t scratch_bytes);
 } // namespace wsp::paged

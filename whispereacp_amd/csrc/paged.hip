@@ -1,19 +1,15 @@
-// The paged cache's kernels: storing new rows, reading rows back, and attention
-// over pages (include/wsp_hip.h, wsp_hip_paged_*). Every address of the pool
-// comes from paged_plan.h's checked lookups.
-#include "device_common.h"
+// The paged cache's rows: storing new ones and reading them back
+// (include/wsp_hip.h, wsp_hip_paged_append and wsp_hip_paged_read). Every address
+// of the pool comes from paged_plan.h's checked look-ups.
 #include "paged.h"
-#include "paged_plan.h"
-
-#include <cmath>
+#include "paged_device.h"
 
 namespace wsp::paged
 {
 namespace
 {
 constexpr int kBlock = 256;
-constexpr int kE4M3 = WSP_E4M3;
-constexpr int kMinExponent = -80, kMaxExponent = 120, kExponentBias = 127;
+constexpr int kMinExponent = -80, kMaxExponent = 120;
 
 // The power of two of an E4M3 row: the least k in range with amax <= 448·2^k
 // (448 = 1.75·2^8).
@@ -89,29 +85,6 @@ __device__ __forceinline__ void store_stored4(void* pool, size_t index, const fl
     }
     else
         *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(pool) + index) = to_e4m3(v, k);
-}
-
-// What the kernels take of a cache and its rows.
-struct Cache
-{
-    int pages, page_shift, heads, head_width;
-    void* keys;
-    void* values;
-    uint8_t* key_exponents;
-    uint8_t* value_exponents;
-};
-struct Rows
-{
-    int sequences, rows, max_count, max_length, table_width;
-    const int* starts;
-    const int* lengths;
-    const int* pages;
-};
-
-__device__ __forceinline__ int page_at(const Cache& cache, const Rows& rows, int sequence, int position)
-{
-    return page_of(rows.pages + (size_t) sequence * rows.table_width, rows.table_width, cache.page_shift, cache.pages,
-                   position);
 }
 
 // ---------------------------------------------------------------------------
@@ -222,134 +195,6 @@ __global__ void __launch_bounds__(kBlock) read_kernel(Cache cache, Rows rows, fl
     *reinterpret_cast<float4u*>(values + (size_t) row * value_stride + (size_t) head * cache.head_width + c) = v;
 }
 
-// ---------------------------------------------------------------------------
-// Attention: a block for each (packed row, query head), 16 groups of 16 lanes,
-// each with every sixteenth key it sees: eight channels a lane, an online
-// softmax (the running maximum and sum, the row rescaled when the maximum
-// grows) a group, and the groups merged through LDS.
-// ---------------------------------------------------------------------------
-template <int ST>
-__global__ void __launch_bounds__(kBlock) row_attention_kernel(Cache cache, Rows rows, const float* __restrict__ q,
-                                                               int q_stride, int heads, int causal, float scale,
-                                                               float* __restrict__ out, int out_stride)
-{
-    constexpr int kGroups = kBlock / 16;
-    __shared__ float tops[kGroups], totals[kGroups];
-    __shared__ float sums[kGroups][kMaxHeadWidth];
-
-    const int row = blockIdx.x / heads, head = blockIdx.x % heads;
-    const int cached = head / (heads / cache.heads), width = cache.head_width;
-    const int sequence = sequence_of(rows.starts, rows.sequences, row);
-    if (sequence < 0 || row - rows.starts[sequence] >= rows.max_count)
-        return;
-    const int length = rows.lengths[sequence];
-    const long long position = position_of(rows.starts, rows.lengths, sequence, row);
-    const int seen = position < 0 ? 0 : causal ? (int) position + 1 : length;
-
-    const int group = threadIdx.x / 16, c = 8 * (threadIdx.x % 16);
-    const bool inside = c < width;
-    const float4v none = {0.f, 0.f, 0.f, 0.f};
-    float4v q0 = none, q1 = none, o0 = none, o1 = none;
-    if (inside)
-    {
-        const float* at = q + (size_t) row * q_stride + (size_t) head * width + c;
-        q0 = *reinterpret_cast<const float4u*>(at);
-        q1 = *reinterpret_cast<const float4u*>(at + 4);
-    }
-    float m = -INFINITY, l = 0.f;
-    if (length > rows.max_length)
-        l = __builtin_nanf("");
-    else
-        for (int j = group; j < seen; j += kGroups)
-        {
-            const int page = page_at(cache, rows, sequence, j);
-            if (page < 0)
-            {
-                l = __builtin_nanf("");
-                break;
-            }
-            const size_t slot = pool_row(page, cached, j & ((1 << cache.page_shift) - 1), cache.heads,
-                                         cache.page_shift);
-            float4v k0 = none, k1 = none, v0 = none, v1 = none;
-            if (inside)
-            {
-                k0 = load_stored4<ST>(cache.keys, slot * width + c);
-                k1 = load_stored4<ST>(cache.keys, slot * width + c + 4);
-                v0 = load_stored4<ST>(cache.values, slot * width + c);
-                v1 = load_stored4<ST>(cache.values, slot * width + c + 4);
-            }
-            float s = 0.f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                s += q0[i] * k0[i] + q1[i] * k1[i];
-            s = sum16(s) * scale;
-            if (s == -INFINITY)
-                continue; // (weight zero; against a maximum of -inf it would be NaN)
-            float gain = 1.f;
-            if constexpr (ST == kE4M3)
-            {
-                s = ldexpf(s, (int) cache.key_exponents[slot] - kExponentBias);
-                gain = ldexpf(1.f, (int) cache.value_exponents[slot] - kExponentBias);
-            }
-            const float top = fmaxf(m, s);
-            const float rescale = expf(m - top), p = expf(s - top);
-            l = l * rescale + p;
-            o0 = o0 * rescale + v0 * (p * gain);
-            o1 = o1 * rescale + v1 * (p * gain);
-            m = top;
-        }
-    if (threadIdx.x % 16 == 0)
-    {
-        tops[group] = m;
-        totals[group] = l;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-    {
-        sums[group][c + i] = o0[i];
-        sums[group][c + 4 + i] = o1[i];
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < width; i += kBlock)
-    {
-        float largest = -INFINITY;
-        for (int w = 0; w < kGroups; ++w)
-            largest = fmaxf(largest, tops[w]);
-        float numerator = 0.f, denominator = 0.f;
-        for (int w = 0; w < kGroups; ++w)
-            if (totals[w] != 0.f) // (a group without a key)
-            {
-                const float factor = expf(tops[w] - largest);
-                numerator += factor * sums[w][i];
-                denominator += factor * totals[w];
-            }
-        out[(size_t) row * out_stride + (size_t) head * width + i] = denominator == 0.f ? 0.f : numerator / denominator;
-    }
-}
-
-Cache device_cache(const wsp_paged_cache& c)
-{
-    return {c.pages, shift_of(c.page_rows), c.heads, c.head_width, c.keys, c.values, c.key_exponents, c.value_exponents};
-}
-
-Rows device_rows(const wsp_paged_rows& r)
-{
-    return {r.sequences, r.rows, r.max_count, r.max_length, r.table_width, r.starts, r.lengths, r.pages};
-}
-
-// f called with the storage as a compile-time constant.
-template <class F>
-void by_storage(int storage, F&& f)
-{
-    switch (storage)
-    {
-        case WSP_F32: return f(std::integral_constant<int, kF32> {});
-        case WSP_F16: return f(std::integral_constant<int, kF16> {});
-        case WSP_BF16: return f(std::integral_constant<int, kBF16> {});
-        default: return f(std::integral_constant<int, kE4M3> {});
-    }
-}
-
 // The same with the storage and the lanes of a (row, head).
 template <class F>
 void by_lanes(const wsp_paged_cache& cache, F&& f)
@@ -383,16 +228,6 @@ hipError_t read(hipStream_t stream, const wsp_paged_cache& cache, const wsp_page
     by_lanes(cache, [&](auto storage, auto lanes) {
         read_kernel<storage(), lanes()><<<row_blocks(cache, rows), kBlock, 0, stream>>>(
             device_cache(cache), device_rows(rows), keys, key_stride, values, value_stride);
-    });
-    return hipGetLastError();
-}
-
-hipError_t attention(hipStream_t stream, const wsp_paged_cache& cache, const wsp_paged_rows& rows, const float* q,
-                     int q_stride, int heads, bool causal, float scale, float* out, int out_stride)
-{
-    by_storage(cache.storage, [&](auto storage) {
-        row_attention_kernel<storage()><<<(unsigned) (rows.rows * heads), kBlock, 0, stream>>>(
-            device_cache(cache), device_rows(rows), q, q_stride, heads, causal, scale, out, out_stride);
     });
     return hipGetLastError();
 }

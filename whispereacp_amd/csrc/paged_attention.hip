@@ -1,0 +1,814 @@
+// Attention over the pages of a cache (include/wsp_hip.h,
+// wsp_hip_paged_attention), on the matrix cores.
+#include "paged.h"
+#include "paged_device.h"
+
+#include <algorithm>
+
+namespace wsp::paged
+{
+namespace
+{
+// What a call asks, beside the cache and the rows.
+struct Query
+{
+    const float* q;
+    int q_stride;
+    int heads, group; // group: query heads a cached head serves
+    int causal;
+    float scale; // times log2(e): the softmax runs in powers of two
+    float* out;
+    int out_stride;
+};
+
+// How a call's keys are split: `splits` blocks of `span` keys each take a row
+// tile's keys, and their partial rows lie at [tile unit][split][row slot].
+struct Split
+{
+    int splits, span, row_slots;
+    float* partials;
+};
+
+// The rows one block computes: for one sequence and one cached head, `tile`
+// consecutive (new row, query head of the group) pairs, row-major.
+struct RowTile
+{
+    int first_row;   // the sequence's first packed row
+    int pairs;       // rows to compute times group
+    int past;        // position of the first new row (before 0: none)
+    int length;
+    int first, last; // this tile's pairs
+    int least, most; // keys that its first and its last row see
+    bool poisoned;   // the length passes max_length
+};
+
+__device__ __forceinline__ int keys_seen(const Query& query, const RowTile& t, int pair)
+{
+    const long long position = (long long) t.past + pair / query.group;
+    return position < 0 ? 0 : query.causal ? (int) position + 1 : t.length;
+}
+
+// False where the tile has no row.
+__device__ __forceinline__ bool find_tile(const Rows& rows, const Query& query, int sequence, int tile, int tile_rows,
+                                          RowTile& t)
+{
+    t.first_row = rows.starts[sequence];
+    const int end = rows.starts[sequence + 1];
+    if (t.first_row < 0 || end <= t.first_row)
+        return false;
+    const int count = end - t.first_row;
+    t.length = rows.lengths[sequence];
+    t.past = max(t.length, 0) - count;
+    t.pairs = min(min(count, rows.max_count), rows.rows - t.first_row) * query.group;
+    t.first = tile * tile_rows;
+    t.last = min(t.first + tile_rows, t.pairs) - 1;
+    if (t.last < t.first)
+        return false;
+    t.poisoned = t.length > rows.max_length;
+    t.least = keys_seen(query, t, t.first);
+    t.most = keys_seen(query, t, t.last);
+    return true;
+}
+
+// Blocks whose keys some row of the tile sees.
+__device__ __forceinline__ int splits_used(const RowTile& t, int span)
+{
+    return t.poisoned ? 1 : max(1, (t.most + span - 1) / span);
+}
+
+__device__ __forceinline__ float* partial_row(const Split& split, int unit, int which, int slot, int width)
+{
+    return split.partials + (((size_t) unit * split.splits + which) * split.row_slots + slot) * (width + 2);
+}
+
+// The largest over the four 16-lane groups, in each of their lanes.
+__device__ __forceinline__ float groups_max(float v)
+{
+    const uint32_t row = __float_as_uint(v);
+    const auto rows = __builtin_amdgcn_permlane16_swap(row, row, false, false);
+    v = fmaxf(__uint_as_float((uint32_t) rows[0]), __uint_as_float((uint32_t) rows[1]));
+    const uint32_t half = __float_as_uint(v);
+    const auto halves = __builtin_amdgcn_permlane32_swap(half, half, false, false);
+    return fmaxf(__uint_as_float((uint32_t) halves[0]), __uint_as_float((uint32_t) halves[1]));
+}
+
+__device__ __forceinline__ float groups_sum(float v)
+{
+    const uint32_t row = __float_as_uint(v);
+    const auto rows = __builtin_amdgcn_permlane16_swap(row, row, false, false);
+    v = __uint_as_float((uint32_t) rows[0]) + __uint_as_float((uint32_t) rows[1]);
+    const uint32_t half = __float_as_uint(v);
+    const auto halves = __builtin_amdgcn_permlane32_swap(half, half, false, false);
+    return __uint_as_float((uint32_t) halves[0]) + __uint_as_float((uint32_t) halves[1]);
+}
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32u __attribute__((aligned(1)));
+
+// Two E4M3 bytes (the low or high half of `packed`) as two fp16, exact.
+template <bool HIGH>
+__device__ __forceinline__ uint32_t e4m3_to_halves(uint32_t packed)
+{
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) packed, 1.f, HIGH));
+}
+
+// What the matrix cores multiply a storage as, and its bytes.
+template <int ST>
+constexpr int operand_of = ST == kE4M3 ? (int) kF16 : ST;
+template <int ST>
+constexpr int bytes_of = ST == kF32 ? 4 : ST == kE4M3 ? 1 : 2;
+
+// Two fp32 values as 16-bit parts packed in dwords: their sum is within 2^-22 of
+// each (two fp16 parts) or exact (three bf16 parts).
+template <int OT>
+__device__ __forceinline__ void cut_pair(float a, float b, uint32_t (&parts)[3])
+{
+    if constexpr (OT == kF16)
+    {
+        typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+        const half2v high = {(_Float16) a, (_Float16) b};
+        const half2v low = {(_Float16) (a - (float) high[0]), (_Float16) (b - (float) high[1])};
+        parts[0] = __builtin_bit_cast(uint32_t, high);
+        parts[1] = __builtin_bit_cast(uint32_t, low);
+    }
+    else
+    {
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+        {
+            const bf16x2 high = {(__bf16) a, (__bf16) b};
+            parts[p] = __builtin_bit_cast(uint32_t, high);
+            a -= (float) high[0];
+            b -= (float) high[1];
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: attention of a tile of 16·QT pairs (new row, head of the group) over
+// keys [split·span, +span) of one cached head, as query_attention_kernel does it
+// for contiguous fp32 caches: a wave takes 32 keys at a time straight from
+// memory into operand registers, with no barrier in the loop, and keeps an
+// online (maximum, sum, row) of each pair; the waves are merged through LDS.
+//
+// S^T = K·Q^T leaves lane (li, g) with keys 4g + r (r < 4) of each 16 and pair li,
+// which is the operand order of O^T = V^T·P^T when the product's eight keys of
+// lane group g are those 4g + r of both sixteens: nothing crosses lanes. A value
+// operand wants eight keys of one channel, and a row in memory holds channels of
+// one key: lane li reads W / 16 channels of its group's eight keys and pairs the
+// halves up itself (v_perm).
+//
+// q, and the weights, go in 16-bit parts (cut_pair), so a product with what the
+// storage holds is as exact as fp32's; fp16 parts of q are of q·2^-e, e from the
+// pair's largest magnitude, and the weights are exp2(s - max + 14), which puts
+// both far from fp16's ends. An E4M3 value row's power of two 2^v would take a
+// weight past them, so the maximum is that of s + v and the parts those of
+// exp2(s + v - max + 14); the sum takes the weights times 2^-v. fp32 storage runs
+// in fp32.
+//
+// Bound by the cache's read where rows are few: a wave keeps the next 32 keys and
+// values in flight while it works on these.
+// ---------------------------------------------------------------------------
+constexpr int kKeys = 32;
+
+template <int ST, int W>
+struct Tile // one lane's part of 32 keys and values, as stored
+{
+    uint32_t k[2][W / 4 * bytes_of<ST> / 4];    // key 16b + li, channels W / 4·g on
+    uint32_t v[2][4][W / 16 * bytes_of<ST> / 4]; // value 16b + 4g + r, channels W / 16·li on
+    uint32_t ke[2], ve[2];                       // E4M3: the exponents of rows 16b + 4g .. + 3
+    bool bad[2];                                 // the page of keys 16b .. is none
+};
+
+template <int WORDS>
+__device__ __forceinline__ void load_words(const char* at, uint32_t (&words)[WORDS])
+{
+    if constexpr (WORDS == 1)
+        words[0] = *global(reinterpret_cast<const uint32_t*>(at));
+    else if constexpr (WORDS == 2)
+    {
+        const u32x2 v = *global(reinterpret_cast<const u32x2*>(at));
+        words[0] = v[0];
+        words[1] = v[1];
+    }
+    else
+    {
+        static_assert(WORDS % 4 == 0);
+#pragma unroll
+        for (int i = 0; i < WORDS / 4; ++i)
+        {
+            const u32x4 v = global(reinterpret_cast<const u32x4*>(at))[i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                words[4 * i + j] = v[j];
+        }
+    }
+}
+
+// Keys k0 .. k0 + 31 of a cached head; k0 is below `end`, and of a sixteen that
+// begins at or past it the first sixteen is read again (nothing there counts).
+template <int ST, int W, bool FULL>
+__device__ __forceinline__ void load_tile(const Cache& cache, const int* table, int table_width, int head, int k0,
+                                          int end, Tile<ST, W>& t)
+{
+    const int lane = threadIdx.x % kWave, li = lane % 16, g = lane / 16;
+    const int mask = (1 << cache.page_shift) - 1, row_bytes = cache.head_width * bytes_of<ST>;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+    {
+        const int from = k0 + 16 * b < end ? k0 + 16 * b : k0;
+        const int page = page_of(table, table_width, cache.page_shift, cache.pages, from);
+        t.bad[b] = page < 0;
+        const size_t row = pool_row(max(page, 0), head, from & mask, cache.heads, cache.page_shift);
+        const char* keys = static_cast<const char*>(cache.keys) + row * row_bytes;
+        const char* values = static_cast<const char*>(cache.values) + row * row_bytes;
+        constexpr int kWords = W / 4 * bytes_of<ST> / 4;
+        if constexpr (FULL)
+            load_words(keys + li * row_bytes + g * (4 * kWords), t.k[b]);
+        else // (a run of 16 bytes lies in the row or past it)
+#pragma unroll
+            for (int i = 0; i < kWords; i += 4)
+            {
+                uint32_t run[4] = {0, 0, 0, 0};
+                if (4 * (g * kWords + i) < row_bytes)
+                    load_words(keys + li * row_bytes + 4 * (g * kWords + i), run);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    t.k[b][i + j] = run[j];
+            }
+        // (Lanes past the row read its start: they hold channels nobody stores.)
+        const int channel = FULL || li * (W / 16) < cache.head_width ? li * (W / 16) : 0;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            load_words(values + (4 * g + r) * row_bytes + channel * bytes_of<ST>, t.v[b][r]);
+        if constexpr (ST == kE4M3)
+        {
+            t.ke[b] = *(const __attribute__((address_space(1))) u32u*) (cache.key_exponents + row + 4 * g);
+            t.ve[b] = *(const __attribute__((address_space(1))) u32u*) (cache.value_exponents + row + 4 * g);
+        }
+    }
+}
+
+// Stored key words as operands: eight channels of 16 bits each.
+template <int ST, int W>
+__device__ __forceinline__ u32x4 key_operand(const Tile<ST, W>& t, int b, int j)
+{
+    if constexpr (ST == kE4M3)
+    {
+        const uint32_t x = t.k[b][2 * j], y = t.k[b][2 * j + 1];
+        return u32x4 {e4m3_to_halves<false>(x), e4m3_to_halves<true>(x), e4m3_to_halves<false>(y),
+                      e4m3_to_halves<true>(y)};
+    }
+    else
+        return u32x4 {t.k[b][4 * j], t.k[b][4 * j + 1], t.k[b][4 * j + 2], t.k[b][4 * j + 3]};
+}
+
+// Channels 2i and 2i + 1 of a stored value row, 16 bits each.
+template <int ST, int W>
+__device__ __forceinline__ uint32_t value_pair(const Tile<ST, W>& t, int b, int r, int i)
+{
+    if constexpr (ST == kE4M3)
+        return i % 2 == 0 ? e4m3_to_halves<false>(t.v[b][r][i / 2]) : e4m3_to_halves<true>(t.v[b][r][i / 2]);
+    else
+        return t.v[b][r][i];
+}
+
+// The bits of a dword's 16-bit halves that are finite, of type OT.
+template <int OT>
+__device__ __forceinline__ uint32_t finite_halves(uint32_t pair)
+{
+    constexpr uint32_t kTop = OT == kF16 ? 0x7C00u : 0x7F80u;
+    uint32_t kept = 0;
+    if ((pair & kTop) != kTop)
+        kept |= pair & 0xFFFFu;
+    if ((pair & (kTop << 16)) != kTop << 16)
+        kept |= pair & 0xFFFF0000u;
+    return kept;
+}
+
+// A stored value widened, E4M3 without its row's power.
+template <int ST>
+__device__ __forceinline__ float stored_value(const void* pool, size_t index)
+{
+    if constexpr (ST == kE4M3)
+        return __builtin_amdgcn_cvt_f32_fp8((int) static_cast<const uint8_t*>(pool)[index], 0);
+    else
+        return load1<ST>(pool, index);
+}
+
+template <int W>
+constexpr int waves_of = 512 / W; // 32 KB of LDS for the merge of 16 pairs
+
+template <int ST, int W, bool FULL, int QT>
+__global__ void __launch_bounds__(waves_of<W>* kWave, 2) tile_attention_kernel(Cache cache, Rows rows, Query query,
+                                                                              Split split, int first_tile,
+                                                                              int first_sequence)
+{
+    constexpr int OT = operand_of<ST>, kParts = parts_of<OT>(), kWaves = waves_of<W>, CPL = W / 16;
+    constexpr float kBias = OT == kF16 ? 14.f : 0.f; // the weights' exponent (see above)
+    __shared__ float tops[kWaves][16], totals[kWaves][16];
+    __shared__ float sums[kWaves][16][W];
+
+    const int which = blockIdx.x % split.splits, head = blockIdx.x / split.splits;
+    const int sequence = first_sequence + blockIdx.z;
+    const int tile = first_tile + (int) (gridDim.y - 1 - blockIdx.y); // (the tiles that see most come first)
+    RowTile tl;
+    if (!find_tile(rows, query, sequence, tile, 16 * QT, tl))
+        return;
+    const int used = splits_used(tl, split.span);
+    if (which >= used)
+        return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int lane = threadIdx.x % kWave, li = lane % 16, g = lane / 16;
+    const int width = cache.head_width;
+    const int* table = rows.pages + (size_t) sequence * rows.table_width;
+    const int begin = which * split.span, end = tl.poisoned ? 0 : min(begin + split.span, tl.most);
+
+    // The queries: lane (li, g) holds channels g·W / 4 .. of pair li, as the keys'.
+    uint32_t qp[QT][OT == kF32 ? 1 : kParts][OT == kF32 ? W / 4 : W / 8];
+    float unit[QT]; // the power of two that the parts leave out
+    int seen[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+    {
+        const int pair = tl.first + 16 * t + li;
+        const bool real = pair <= tl.last;
+        seen[t] = real ? min(keys_seen(query, tl, pair), end) : end;
+        float x[W / 4];
+        const float* at = query.q + (size_t) (tl.first_row + (real ? pair : tl.first) / query.group) * query.q_stride
+                          + (size_t) (head * query.group + (real ? pair : tl.first) % query.group) * width;
+#pragma unroll
+        for (int i = 0; i < W / 4; i += 4)
+        {
+            float4v run = {0.f, 0.f, 0.f, 0.f};
+            if (real && (FULL || g * (W / 4) + i < width))
+                run = *reinterpret_cast<const float4u*>(at + g * (W / 4) + i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                x[i + j] = run[j] * query.scale;
+        }
+        unit[t] = 1.f;
+        if constexpr (OT == kF32)
+#pragma unroll
+            for (int i = 0; i < W / 4; ++i)
+                qp[t][0][i] = __float_as_uint(x[i]);
+        else
+        {
+            if constexpr (OT == kF16)
+            {
+                float top = 0.f;
+#pragma unroll
+                for (int i = 0; i < W / 4; ++i)
+                    top = fmaxf(top, fabsf(x[i]));
+                top = groups_max(top);
+                // 2^13 <= top·2^shift < 2^14 (a pair of zeros, or not finite: as it is)
+                int shift = 140 - (int) (__float_as_uint(top) >> 23);
+                shift = top > 0.f && top < INFINITY ? min(shift, 100) : 0;
+#pragma unroll
+                for (int i = 0; i < W / 4; ++i)
+                    x[i] = ldexpf(x[i], shift);
+                unit[t] = ldexpf(1.f, -shift);
+            }
+#pragma unroll
+            for (int i = 0; i < W / 8; ++i)
+            {
+                uint32_t cut[3];
+                cut_pair<OT>(x[2 * i], x[2 * i + 1], cut);
+#pragma unroll
+                for (int p = 0; p < kParts; ++p)
+                    qp[t][p][i] = cut[p];
+            }
+        }
+    }
+
+    float4v o[QT][CPL];
+    float m[QT], l[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+    {
+        m[t] = -INFINITY;
+        l[t] = 0.f;
+#pragma unroll
+        for (int c = 0; c < CPL; ++c)
+            o[t][c] = float4v {0.f, 0.f, 0.f, 0.f};
+    }
+
+    auto work = [&](const Tile<ST, W>& kv, int k0) {
+        // Keys that not every pair sees, or whose page is none, take the careful way.
+        const bool careful = k0 + kKeys > min(tl.least, end) || kv.bad[0] || kv.bad[1];
+        uint32_t weights[QT][OT == kF32 ? 1 : kParts][OT == kF32 ? 8 : 4];
+        float alpha[QT];
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+        {
+            float4v s[2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+            {
+                if constexpr (OT == kF32)
+                {
+                    // Four partial sums a score: short chains of roundings, and products
+                    // that need not wait for each other.
+                    float4v part[4];
+#pragma unroll
+                    for (int i = 0; i < W / 4; ++i)
+                        part[i % 4] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                            __uint_as_float(kv.k[b][i]), __uint_as_float(qp[t][0][i]),
+                            i < 4 ? float4v {0.f, 0.f, 0.f, 0.f} : part[i % 4], 0, 0, 0);
+                    s[b] = (part[0] + part[1]) + (part[2] + part[3]);
+                }
+                else
+                {
+                    float4v part[kParts];
+#pragma unroll
+                    for (int j = 0; j < W / 32; ++j)
+                    {
+                        const u32x4 key = key_operand<ST, W>(kv, b, j);
+#pragma unroll
+                        for (int p = 0; p < kParts; ++p)
+                            part[p] = mfma16<OT>(key,
+                                                 u32x4 {qp[t][p][4 * j], qp[t][p][4 * j + 1], qp[t][p][4 * j + 2],
+                                                        qp[t][p][4 * j + 3]},
+                                                 j == 0 ? float4v {0.f, 0.f, 0.f, 0.f} : part[p]);
+                    }
+                    s[b] = part[kParts - 1];
+#pragma unroll
+                    for (int p = kParts - 2; p >= 0; --p)
+                        s[b] += part[p];
+                }
+            }
+            // Scores in powers of two; E4M3 ones with the value rows' powers in them.
+            float inverse[2][4];
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                {
+                    if constexpr (ST == kE4M3)
+                    {
+                        const uint32_t ke = kv.ke[b] >> (8 * r) & 255u, ve = kv.ve[b] >> (8 * r) & 255u;
+                        s[b][r] = __builtin_fmaf(s[b][r], unit[t] * __uint_as_float(ke << 23),
+                                                 (float) ve - (float) kExponentBias);
+                        inverse[b][r] = __uint_as_float((254u - ve) << 23);
+                    }
+                    else if constexpr (OT == kF16)
+                        s[b][r] *= unit[t];
+                }
+            if (careful)
+            {
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                    {
+                        if (kv.bad[b])
+                            s[b][r] = __builtin_nanf("");
+                        if (ST == kE4M3 && (kv.bad[b] || k0 + 16 * b + 4 * g + r >= end))
+                            inverse[b][r] = 0.f;
+                        s[b][r] = k0 + 16 * b + 4 * g + r < seen[t] ? s[b][r] : -INFINITY;
+                    }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    top = fmaxf(top, s[b][r]);
+            // The maximum is rounded up to a whole power of two, so that what it rescales
+            // and the bias stay exact however often it grows. (Before a key of finite
+            // score, zero in its place: the weights are zero.)
+            const float m_new = fmaxf(m[t], ceilf(groups_max(top)));
+            const float finite = m_new == -INFINITY ? 0.f : m_new, base = finite - kBias;
+            alpha[t] = __builtin_amdgcn_exp2f(m[t] - finite);
+            m[t] = m_new;
+            float own = 0.f;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                {
+                    s[b][r] = __builtin_amdgcn_exp2f(s[b][r] - base);
+                    own += ST == kE4M3 ? s[b][r] * inverse[b][r] : s[b][r];
+                }
+            l[t] = l[t] * alpha[t] + own;
+#pragma unroll
+            for (int i = 0; i < (OT == kF32 ? 8 : 4); ++i)
+                if constexpr (OT == kF32)
+                    weights[t][0][i] = __float_as_uint(s[i / 4][i % 4]);
+                else
+                {
+                    uint32_t cut[3];
+                    cut_pair<OT>(s[i / 2][2 * (i % 2)], s[i / 2][2 * (i % 2) + 1], cut);
+#pragma unroll
+                    for (int p = 0; p < kParts; ++p)
+                        weights[t][p][i] = cut[p];
+                }
+        }
+
+        // The rows, two channels of each lane's at a time. Every 32 keys are summed
+        // on their own and join the row by the multiply-add that rescales it.
+        bool odd = false;
+        const float4v none = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < CPL; c += 2)
+        {
+            // Channels CPL·li + c and + c + 1 of keys 16b + 4g + r. A weight of zero
+            // hides a value only while it is finite: the careful way counts values
+            // that no pair sees as zero, and non-finite ones that some pair sees are
+            // added behind the products, to those pairs alone.
+            if constexpr (OT == kF32)
+            {
+                float v[2][8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        v[e][i] = __uint_as_float(kv.v[i / 4][i % 4][c + e]);
+                if (careful)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                    {
+                        const bool unseen = k0 + 16 * (i / 4) + 4 * g + i % 4 >= end || kv.bad[i / 4];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                        {
+                            odd = odd || (!unseen && !isfinite(v[e][i]));
+                            v[e][i] = unseen || !isfinite(v[e][i]) ? 0.f : v[e][i];
+                        }
+                    }
+#pragma unroll
+                for (int t = 0; t < QT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                    {
+                        float4v part = none;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            part = __builtin_amdgcn_mfma_f32_16x16x4f32(v[e][i], __uint_as_float(weights[t][0][i]),
+                                                                        part, 0, 0, 0);
+                        o[t][c + e] = o[t][c + e] * alpha[t] + part;
+                    }
+            }
+            else
+            {
+                u32x4 v[2];
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+                {
+                    const uint32_t x = value_pair<ST, W>(kv, d / 2, 2 * (d % 2), c / 2);
+                    const uint32_t y = value_pair<ST, W>(kv, d / 2, 2 * (d % 2) + 1, c / 2);
+                    v[0][d] = __builtin_amdgcn_perm(y, x, 0x05040100); // the low halves
+                    v[1][d] = __builtin_amdgcn_perm(y, x, 0x07060302); // the high ones
+                }
+                if (careful)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                    {
+                        const bool unseen = k0 + 16 * (i / 4) + 4 * g + i % 4 >= end || kv.bad[i / 4];
+                        const uint32_t half = i % 2 == 0 ? 0xFFFFu : 0xFFFF0000u;
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                        {
+                            const uint32_t kept = unseen ? 0u : finite_halves<OT>(v[e][i / 2] & half);
+                            odd = odd || (!unseen && kept != (v[e][i / 2] & half));
+                            v[e][i / 2] = (v[e][i / 2] & ~half) | kept;
+                        }
+                    }
+#pragma unroll
+                for (int t = 0; t < QT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                    {
+                        float4v part = none;
+#pragma unroll
+                        for (int p = kParts - 1; p >= 0; --p)
+                            part = mfma16<OT>(v[e],
+                                              u32x4 {weights[t][p][0], weights[t][p][1], weights[t][p][2],
+                                                     weights[t][p][3]},
+                                              part);
+                        o[t][c + e] = o[t][c + e] * alpha[t] + part;
+                    }
+            }
+        }
+        if (careful && __any(odd)) // (rare: infinities or NaN among the new rows' values)
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+#pragma unroll 1
+                for (int key = 0; key < kKeys; ++key)
+                {
+                    // Key 16b + 4g + r is held by lane group g. (Only that its weight is
+                    // not zero matters: the first part of it does.)
+                    const int at = 4 * (key / 16) + key % 4;
+                    uint32_t pair = 0;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (i == at)
+                            pair = weights[t][0][OT == kF32 ? i : i / 2];
+                    const uint32_t held = OT == kF32 ? pair : at % 2 == 0 ? pair << 16 : pair & 0xFFFF0000u;
+                    const float weight = __uint_as_float(__shfl(held, li + 16 * (key / 4 % 4)));
+                    const int position = k0 + key;
+                    const int page = page_of(table, rows.table_width, cache.page_shift, cache.pages, position);
+                    if (position >= seen[t] || page < 0)
+                        continue;
+                    const size_t row = pool_row(page, head, position & ((1 << cache.page_shift) - 1), cache.heads,
+                                                cache.page_shift);
+#pragma unroll
+                    for (int c = 0; c < CPL; ++c)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                        {
+                            const int channel = (4 * g + r) * CPL + c;
+                            const float value =
+                                channel < width ? stored_value<ST>(cache.values, row * width + channel) : 0.f;
+                            if (!isfinite(value))
+                                o[t][c][r] += weight * value;
+                        }
+                }
+    };
+
+    constexpr int kStride = kKeys * kWaves;
+    int k0 = begin + kKeys * wave;
+    if (k0 < end)
+    {
+        Tile<ST, W> now;
+        load_tile<ST, W, FULL>(cache, table, rows.table_width, head, k0, end, now);
+        for (; k0 + kStride < end; k0 += kStride)
+        {
+            Tile<ST, W> next;
+            load_tile<ST, W, FULL>(cache, table, rows.table_width, head, k0 + kStride, end, next);
+            __builtin_amdgcn_sched_barrier(0);
+            work(now, k0);
+            now = next;
+        }
+        work(now, k0);
+    }
+
+    // The waves merged, 16 pairs at a time. o[t][c][r] is channel CPL·(4g + r) + c of pair li.
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+    {
+        const float total = groups_sum(l[t]);
+        if (t > 0)
+            __syncthreads(); // (the rows before are read)
+        if (g == 0)
+        {
+            tops[wave][li] = m[t];
+            totals[wave][li] = total;
+        }
+        if (tl.first + 16 * t + li <= tl.last)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int c = 0; c < CPL; c += 4)
+                    *reinterpret_cast<float4v*>(&sums[wave][li][CPL * (4 * g + r) + c]) =
+                        float4v {o[t][c][r], o[t][c + 1][r], o[t][c + 2][r], o[t][c + 3][r]};
+        __syncthreads();
+        for (int i = threadIdx.x; i < 16 * W; i += kWaves * kWave)
+        {
+            const int at = i / W, c = i % W, pair = tl.first + 16 * t + at;
+            if (pair > tl.last || (!FULL && c >= width))
+                continue;
+            float largest = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w)
+                largest = fmaxf(largest, tops[w][at]);
+            float numerator = 0.f, denominator = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w)
+                if (totals[w][at] != 0.f) // (a wave without a key)
+                {
+                    const float factor = __builtin_amdgcn_exp2f(tops[w][at] - largest);
+                    numerator += factor * sums[w][at][c];
+                    denominator += factor * totals[w][at];
+                }
+            if (tl.poisoned)
+                numerator = denominator = __builtin_nanf("");
+            if (used == 1)
+                query.out[(size_t) (tl.first_row + pair / query.group) * query.out_stride
+                          + (size_t) (head * query.group + pair % query.group) * width + c] =
+                    denominator == 0.f ? 0.f : numerator / denominator;
+            else
+            {
+                const int unit_index = ((int) blockIdx.z * (int) gridDim.y + (int) blockIdx.y) * cache.heads + head;
+                float* part = partial_row(split, unit_index, which, 16 * t + at, width);
+                part[2 + c] = numerator;
+                if (c == 0)
+                {
+                    part[0] = largest;
+                    part[1] = denominator;
+                }
+            }
+        }
+    }
+}
+
+// The partial rows of a pair's splits joined: a block for each (pair, cached
+// head, tile, sequence) of the launch before, whose grid this one's y and z
+// repeat. Its four waves take every fourth split, several in flight.
+constexpr int kJoinWaves = 4;
+
+__global__ void __launch_bounds__(kJoinWaves* kWave) join_kernel(Cache cache, Rows rows, Query query, Split split,
+                                                                 int tile_rows, int first_tile, int first_sequence)
+{
+    __shared__ float sums[kJoinWaves][kMaxHeadWidth], totals[kJoinWaves];
+    const int slot = blockIdx.x % split.row_slots, head = blockIdx.x / split.row_slots;
+    RowTile tl;
+    if (!find_tile(rows, query, first_sequence + blockIdx.z, first_tile + (int) (gridDim.y - 1 - blockIdx.y), tile_rows,
+                   tl))
+        return;
+    const int pair = tl.first + slot, used = splits_used(tl, split.span);
+    if (pair > tl.last || used == 1)
+        return;
+    const int width = cache.head_width, wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    const int unit_index = ((int) blockIdx.z * (int) gridDim.y + (int) blockIdx.y) * cache.heads + head;
+    const float* first = partial_row(split, unit_index, 0, slot, width);
+    const size_t pitch = (size_t) split.row_slots * (width + 2);
+
+    float largest = -INFINITY;
+    for (int i = lane; i < used; i += kWave)
+        largest = fmaxf(largest, first[i * pitch]);
+    largest = wave_max(largest);
+
+    const int c0 = min(lane, width - 1), c1 = min(lane + kWave, width - 1);
+    float low = 0.f, high = 0.f, denominator = 0.f;
+#pragma unroll 4
+    for (int i = wave; i < used; i += kJoinWaves)
+    {
+        const float* part = first + i * pitch;
+        const float top = part[0], total = part[1], a = part[2 + c0], b = part[2 + c1];
+        if (total != 0.f) // (a split without a key of finite score)
+        {
+            const float factor = __builtin_amdgcn_exp2f(top - largest);
+            low += factor * a;
+            high += factor * b;
+            denominator += factor * total;
+        }
+    }
+    sums[wave][lane] = low;
+    sums[wave][lane + kWave] = high;
+    if (lane == 0)
+        totals[wave] = denominator;
+    __syncthreads();
+    for (int c = threadIdx.x; c < width; c += kJoinWaves * kWave)
+    {
+        float numerator = 0.f, total = 0.f;
+#pragma unroll
+        for (int w = 0; w < kJoinWaves; ++w)
+        {
+            numerator += sums[w][c];
+            total += totals[w];
+        }
+        query.out[(size_t) (tl.first_row + pair / query.group) * query.out_stride
+                  + (size_t) (head * query.group + pair % query.group) * width + c] =
+            total == 0.f ? 0.f : numerator / total;
+    }
+}
+
+constexpr int kMostBlocks = 65535; // of a launch's y and z extents
+
+template <int ST, int W, bool FULL, int QT>
+void launch_tiles(hipStream_t stream, const Cache& cache, const Rows& rows, const Query& query, const Plan& plan,
+                  const Split& split)
+{
+    for (int s = 0; s < rows.sequences; s += plan.slice)
+        for (int t = 0; t < plan.tiles; t += kMostBlocks)
+        {
+            const dim3 grid(split.splits * cache.heads, std::min(plan.tiles - t, kMostBlocks),
+                            std::min(rows.sequences - s, plan.slice));
+            tile_attention_kernel<ST, W, FULL, QT>
+                <<<grid, waves_of<W> * kWave, 0, stream>>>(cache, rows, query, split, t, s);
+            if (split.splits > 1)
+                join_kernel<<<dim3(cache.heads * split.row_slots, grid.y, grid.z), kJoinWaves * kWave, 0, stream>>>(
+                    cache, rows, query, split, 16 * QT, t, s);
+        }
+}
+} // namespace
+
+hipError_t attention(hipStream_t stream, const wsp_paged_cache& cache, const wsp_paged_rows& rows, const float* q,
+                     int q_stride, int heads, bool causal, float scale, float* out, int out_stride, void* scratch,
+                     size_t scratch_bytes)
+{
+    if (rows.max_count == 0)
+        return hipSuccess;
+    const Query query {q, q_stride, heads, heads / cache.heads, causal, scale * 1.4426950408889634f, out, out_stride};
+    const Plan plan = plan_attention(rows, cache.heads, query.group, cache.head_width, scratch_bytes / sizeof(float));
+    const Split split {plan.splits, plan.span, plan.row_slots, static_cast<float*>(scratch)};
+    by_storage(cache.storage, [&](auto storage) {
+        auto run = [&](auto width, auto full) {
+            plan.tile_rows == 16
+                ? launch_tiles<storage(), width(), full(), 1>(stream, device_cache(cache), device_rows(rows), query,
+                                                              plan, split)
+                : launch_tiles<storage(), width(), full(), 2>(stream, device_cache(cache), device_rows(rows), query,
+                                                              plan, split);
+        };
+        using Narrow = std::integral_constant<int, 64>;
+        using Wide = std::integral_constant<int, 128>;
+        cache.head_width == 64    ? run(Narrow {}, std::true_type {})
+        : cache.head_width == 128 ? run(Wide {}, std::true_type {})
+        : cache.head_width < 64   ? run(Narrow {}, std::false_type {})
+                                  : run(Wide {}, std::false_type {});
+    });
+    return hipGetLastError();
+}
+} // namespace wsp::paged

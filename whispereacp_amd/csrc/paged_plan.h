@@ -80,6 +80,44 @@ inline int say(char* why, size_t size, int code, const char* format, ...)
     return code;
 }
 
+// How an attention call is cut: blocks of tile_rows pairs (new row, query head
+// of a cached head's group), `splits` blocks of `span` keys along the keys, and
+// launches of at most `slice` sequences. Splits leave partial rows of
+// head_width + 2 floats, row_slots to a block, in a scratch of scratch_floats.
+struct Plan
+{
+    int tile_rows, tiles;
+    int splits, span, row_slots;
+    int slice;
+};
+
+constexpr int kWantedBlocks = 2048; // eight a CU: lengths differ, and shorter sequences' blocks end early
+constexpr int kLeastSpan = 256;     // keys a block's waves take at once
+constexpr int kMostSequences = 65535; // a launch's z extent
+
+inline Plan plan_attention(const wsp_paged_rows& rows, int heads, int group, int head_width, size_t scratch_floats)
+{
+    Plan plan {};
+    const long long pairs = (long long) rows.max_count * group;
+    plan.tile_rows = pairs <= 16 ? 16 : 32;
+    plan.tiles = (int) ((pairs + plan.tile_rows - 1) / plan.tile_rows);
+    plan.row_slots = (int) (pairs < plan.tile_rows ? pairs : plan.tile_rows);
+    plan.slice = rows.sequences < kMostSequences ? rows.sequences : kMostSequences;
+    const long long units = (long long) plan.tiles * heads * plan.slice;
+    const size_t unit_floats = (size_t) plan.row_slots * (head_width + 2);
+    long long splits = (rows.max_length + kLeastSpan - 1) / kLeastSpan;
+    if (splits > kWantedBlocks / units)
+        splits = kWantedBlocks / units;
+    if ((unsigned long long) splits > scratch_floats / unit_floats / units)
+        splits = (long long) (scratch_floats / unit_floats / units);
+    if (splits < 2)
+        splits = 1;
+    plan.span = (int) ((rows.max_length + splits - 1) / splits);
+    plan.span = plan.span < kLeastSpan ? kLeastSpan : (plan.span + 31) / 32 * 32;
+    plan.splits = rows.max_length <= plan.span ? 1 : (rows.max_length + plan.span - 1) / plan.span;
+    return plan;
+}
+
 // Why a call over this cache and these rows is refused: WSP_OK, or a status
 // with the reason in `why`.
 inline int refusal(const wsp_paged_cache* cache, const wsp_paged_rows* rows, char* why, size_t size)
