@@ -175,7 +175,7 @@ constexpr int kKeys = 32;
 template <int ST, int W>
 struct Tile // one lane's part of 32 keys and values, as stored
 {
-    uint32_t k[2][W / 4 * bytes_of<ST> / 4];    // key 16b + li, channels W / 4·g on
+    uint32_t k[2][W / 4 * bytes_of<ST> / 4];     // key 16b + li, 16-byte runs g, g + 4, ... of the row
     uint32_t v[2][4][W / 16 * bytes_of<ST> / 4]; // value 16b + 4g + r, channels W / 16·li on
     uint32_t ke[2], ve[2];                       // E4M3: the exponents of rows 16b + 4g .. + 3
     bool bad[2];                                 // the page of keys 16b .. is none
@@ -206,37 +206,49 @@ __device__ __forceinline__ void load_words(const char* at, uint32_t (&words)[WOR
     }
 }
 
-// Keys k0 .. k0 + 31 of a cached head; k0 is below `end`, and of a sixteen that
-// begins at or past it the first sixteen is read again (nothing there counts).
+// The pages of keys k0 .. k0 + 15 and k0 + 16 .. k0 + 31 (-1: none). k0 is below
+// `end`; of a sixteen that begins at or past it the first is named again (nothing
+// there counts).
+struct Pages
+{
+    int page[2];
+};
+__device__ __forceinline__ int second_key(int k0, int end)
+{
+    return k0 + 16 < end ? k0 + 16 : k0;
+}
+__device__ __forceinline__ Pages find_pages(const Cache& cache, const int* table, int table_width, int k0, int end)
+{
+    return {{page_of(table, table_width, cache.page_shift, cache.pages, k0),
+             page_of(table, table_width, cache.page_shift, cache.pages, second_key(k0, end))}};
+}
+
+// Keys and values k0 .. k0 + 31 of a cached head.
 template <int ST, int W, bool FULL>
-__device__ __forceinline__ void load_tile(const Cache& cache, const int* table, int table_width, int head, int k0,
-                                          int end, Tile<ST, W>& t)
+__device__ __forceinline__ void load_tile(const Cache& cache, const Pages& pages, int head, int k0, int end,
+                                          Tile<ST, W>& t)
 {
     const int lane = threadIdx.x % kWave, li = lane % 16, g = lane / 16;
     const int mask = (1 << cache.page_shift) - 1, row_bytes = cache.head_width * bytes_of<ST>;
 #pragma unroll
     for (int b = 0; b < 2; ++b)
     {
-        const int from = k0 + 16 * b < end ? k0 + 16 * b : k0;
-        const int page = page_of(table, table_width, cache.page_shift, cache.pages, from);
-        t.bad[b] = page < 0;
-        const size_t row = pool_row(max(page, 0), head, from & mask, cache.heads, cache.page_shift);
+        t.bad[b] = pages.page[b] < 0;
+        const size_t row = pool_row(max(pages.page[b], 0), head, (b == 0 ? k0 : second_key(k0, end)) & mask, cache.heads,
+                                    cache.page_shift);
         const char* keys = static_cast<const char*>(cache.keys) + row * row_bytes;
         const char* values = static_cast<const char*>(cache.values) + row * row_bytes;
-        constexpr int kWords = W / 4 * bytes_of<ST> / 4;
-        if constexpr (FULL)
-            load_words(keys + li * row_bytes + g * (4 * kWords), t.k[b]);
-        else // (a run of 16 bytes lies in the row or past it)
+        constexpr int kRuns = W * bytes_of<ST> / 64;
 #pragma unroll
-            for (int i = 0; i < kWords; i += 4)
-            {
-                uint32_t run[4] = {0, 0, 0, 0};
-                if (4 * (g * kWords + i) < row_bytes)
-                    load_words(keys + li * row_bytes + 4 * (g * kWords + i), run);
+        for (int i = 0; i < kRuns; ++i) // (a run lies in the row or past it)
+        {
+            uint32_t run[4] = {0, 0, 0, 0};
+            if (FULL || 16 * (4 * i + g) < row_bytes)
+                load_words(keys + li * row_bytes + 16 * (4 * i + g), run);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    t.k[b][i + j] = run[j];
-            }
+            for (int j = 0; j < 4; ++j)
+                t.k[b][4 * i + j] = run[j];
+        }
         // (Lanes past the row read its start: they hold channels nobody stores.)
         const int channel = FULL || li * (W / 16) < cache.head_width ? li * (W / 16) : 0;
 #pragma unroll
@@ -297,15 +309,14 @@ __device__ __forceinline__ float stored_value(const void* pool, size_t index)
         return load1<ST>(pool, index);
 }
 
-template <int W>
-constexpr int waves_of = 512 / W; // 32 KB of LDS for the merge of 16 pairs
+constexpr int kTileWaves = 4;
 
 template <int ST, int W, bool FULL, int QT>
-__global__ void __launch_bounds__(waves_of<W>* kWave, 2) tile_attention_kernel(Cache cache, Rows rows, Query query,
+__global__ void __launch_bounds__(kTileWaves* kWave, 2) tile_attention_kernel(Cache cache, Rows rows, Query query,
                                                                               Split split, int first_tile,
                                                                               int first_sequence)
 {
-    constexpr int OT = operand_of<ST>, kParts = parts_of<OT>(), kWaves = waves_of<W>, CPL = W / 16;
+    constexpr int OT = operand_of<ST>, kParts = parts_of<OT>(), kWaves = kTileWaves, CPL = W / 16;
     constexpr float kBias = OT == kF16 ? 14.f : 0.f; // the weights' exponent (see above)
     __shared__ float tops[kWaves][16], totals[kWaves][16];
     __shared__ float sums[kWaves][16][W];
@@ -325,7 +336,7 @@ __global__ void __launch_bounds__(waves_of<W>* kWave, 2) tile_attention_kernel(C
     const int* table = rows.pages + (size_t) sequence * rows.table_width;
     const int begin = which * split.span, end = tl.poisoned ? 0 : min(begin + split.span, tl.most);
 
-    // The queries: lane (li, g) holds channels g·W / 4 .. of pair li, as the keys'.
+    // The queries: lane (li, g) holds the channels of pair li that it holds of a key.
     uint32_t qp[QT][OT == kF32 ? 1 : kParts][OT == kF32 ? W / 4 : W / 8];
     float unit[QT]; // the power of two that the parts leave out
     int seen[QT];
@@ -341,9 +352,11 @@ __global__ void __launch_bounds__(waves_of<W>* kWave, 2) tile_attention_kernel(C
 #pragma unroll
         for (int i = 0; i < W / 4; i += 4)
         {
+            constexpr int kRun = 16 / bytes_of<ST>;
+            const int channel = (4 * (i / kRun) + g) * kRun + i % kRun;
             float4v run = {0.f, 0.f, 0.f, 0.f};
-            if (real && (FULL || g * (W / 4) + i < width))
-                run = *reinterpret_cast<const float4u*>(at + g * (W / 4) + i);
+            if (real && (FULL || channel < width))
+                run = *reinterpret_cast<const float4u*>(at + channel);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 x[i + j] = run[j] * query.scale;
@@ -627,18 +640,31 @@ __global__ void __launch_bounds__(waves_of<W>* kWave, 2) tile_attention_kernel(C
                 }
     };
 
+    // The next keys are in flight while these are worked on (not where two tiles
+    // do not fit the registers), and the pages of those behind them looked up.
     constexpr int kStride = kKeys * kWaves;
+    constexpr bool kAhead = ST != kF32 || W == 64;
     int k0 = begin + kKeys * wave;
     if (k0 < end)
     {
         Tile<ST, W> now;
-        load_tile<ST, W, FULL>(cache, table, rows.table_width, head, k0, end, now);
+        Pages pages = find_pages(cache, table, rows.table_width, k0, end);
+        load_tile<ST, W, FULL>(cache, pages, head, k0, end, now);
+        if (k0 + kStride < end)
+            pages = find_pages(cache, table, rows.table_width, k0 + kStride, end);
         for (; k0 + kStride < end; k0 += kStride)
         {
+            if constexpr (!kAhead)
+                work(now, k0);
             Tile<ST, W> next;
-            load_tile<ST, W, FULL>(cache, table, rows.table_width, head, k0 + kStride, end, next);
-            __builtin_amdgcn_sched_barrier(0);
-            work(now, k0);
+            load_tile<ST, W, FULL>(cache, pages, head, k0 + kStride, end, next);
+            if (k0 + 2 * kStride < end)
+                pages = find_pages(cache, table, rows.table_width, k0 + 2 * kStride, end);
+            if constexpr (kAhead)
+            {
+                __builtin_amdgcn_sched_barrier(0);
+                work(now, k0);
+            }
             now = next;
         }
         work(now, k0);
@@ -708,6 +734,7 @@ __global__ void __launch_bounds__(waves_of<W>* kWave, 2) tile_attention_kernel(C
 // repeat. Its four waves take every fourth split, several in flight.
 constexpr int kJoinWaves = 4;
 
+template <int AHEAD>
 __global__ void __launch_bounds__(kJoinWaves* kWave) join_kernel(Cache cache, Rows rows, Query query, Split split,
                                                                  int tile_rows, int first_tile, int first_sequence)
 {
@@ -725,6 +752,7 @@ __global__ void __launch_bounds__(kJoinWaves* kWave) join_kernel(Cache cache, Ro
     const float* first = partial_row(split, unit_index, 0, slot, width);
     const size_t pitch = (size_t) split.row_slots * (width + 2);
 
+    // Every wave the largest of all; then a wave each fourth split, eight in flight.
     float largest = -INFINITY;
     for (int i = lane; i < used; i += kWave)
         largest = fmaxf(largest, first[i * pitch]);
@@ -732,18 +760,27 @@ __global__ void __launch_bounds__(kJoinWaves* kWave) join_kernel(Cache cache, Ro
 
     const int c0 = min(lane, width - 1), c1 = min(lane + kWave, width - 1);
     float low = 0.f, high = 0.f, denominator = 0.f;
-#pragma unroll 4
-    for (int i = wave; i < used; i += kJoinWaves)
+    for (int i0 = wave; i0 < used; i0 += AHEAD * kJoinWaves)
     {
-        const float* part = first + i * pitch;
-        const float top = part[0], total = part[1], a = part[2 + c0], b = part[2 + c1];
-        if (total != 0.f) // (a split without a key of finite score)
+        float top[AHEAD], total[AHEAD], a[AHEAD], b[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
         {
-            const float factor = __builtin_amdgcn_exp2f(top - largest);
-            low += factor * a;
-            high += factor * b;
-            denominator += factor * total;
+            const float* part = first + min(i0 + i * kJoinWaves, used - 1) * pitch;
+            top[i] = part[0];
+            total[i] = part[1];
+            a[i] = part[2 + c0];
+            b[i] = part[2 + c1];
         }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (i0 + i * kJoinWaves < used && total[i] != 0.f) // (a split without a key of finite score sums to zero)
+            {
+                const float factor = __builtin_amdgcn_exp2f(top[i] - largest);
+                low += factor * a[i];
+                high += factor * b[i];
+                denominator += factor * total[i];
+            }
     }
     sums[wave][lane] = low;
     sums[wave][lane + kWave] = high;
@@ -777,9 +814,10 @@ void launch_tiles(hipStream_t stream, const Cache& cache, const Rows& rows, cons
             const dim3 grid(split.splits * cache.heads, std::min(plan.tiles - t, kMostBlocks),
                             std::min(rows.sequences - s, plan.slice));
             tile_attention_kernel<ST, W, FULL, QT>
-                <<<grid, waves_of<W> * kWave, 0, stream>>>(cache, rows, query, split, t, s);
+                <<<grid, kTileWaves * kWave, 0, stream>>>(cache, rows, query, split, t, s);
             if (split.splits > 1)
-                join_kernel<<<dim3(cache.heads * split.row_slots, grid.y, grid.z), kJoinWaves * kWave, 0, stream>>>(
+                (split.splits <= kJoinWaves ? join_kernel<1> : join_kernel<8>)<<<
+                    dim3(cache.heads * split.row_slots, grid.y, grid.z), kJoinWaves * kWave, 0, stream>>>(
                     cache, rows, query, split, 16 * QT, t, s);
         }
 }
@@ -792,15 +830,17 @@ hipError_t attention(hipStream_t stream, const wsp_paged_cache& cache, const wsp
     if (rows.max_count == 0)
         return hipSuccess;
     const Query query {q, q_stride, heads, heads / cache.heads, causal, scale * 1.4426950408889634f, out, out_stride};
-    const Plan plan = plan_attention(rows, cache.heads, query.group, cache.head_width, scratch_bytes / sizeof(float));
+    const Plan plan = plan_attention(rows, cache.storage, cache.heads, query.group, cache.head_width,
+                                     scratch_bytes / sizeof(float));
     const Split split {plan.splits, plan.span, plan.row_slots, static_cast<float*>(scratch)};
     by_storage(cache.storage, [&](auto storage) {
         auto run = [&](auto width, auto full) {
-            plan.tile_rows == 16
-                ? launch_tiles<storage(), width(), full(), 1>(stream, device_cache(cache), device_rows(rows), query,
-                                                              plan, split)
-                : launch_tiles<storage(), width(), full(), 2>(stream, device_cache(cache), device_rows(rows), query,
-                                                              plan, split);
+            if constexpr (storage() != kF32 || width() == 64)
+                if (plan.tile_rows == 32)
+                    return launch_tiles<storage(), width(), full(), 2>(stream, device_cache(cache), device_rows(rows),
+                                                                       query, plan, split);
+            launch_tiles<storage(), width(), full(), 1>(stream, device_cache(cache), device_rows(rows), query, plan,
+                                                        split);
         };
         using Narrow = std::integral_constant<int, 64>;
         using Wide = std::integral_constant<int, 128>;

@@ -91,23 +91,28 @@ struct Plan
     int slice;
 };
 
-constexpr int kWantedBlocks = 2048; // eight a CU: lengths differ, and shorter sequences' blocks end early
-constexpr int kLeastSpan = 256;     // keys a block's waves take at once
+constexpr int kRoundBlocks = 768; // blocks that run at once, three a CU
+constexpr int kLeastSpan = 256;   // two turns of a block's waves
+constexpr int kMostSpan = 2048;   // lengths differ: blocks of longer spans end apart
 constexpr int kMostSequences = 65535; // a launch's z extent
 
-inline Plan plan_attention(const wsp_paged_rows& rows, int heads, int group, int head_width, size_t scratch_floats)
+inline Plan plan_attention(const wsp_paged_rows& rows, int storage, int heads, int group, int head_width,
+                           size_t scratch_floats)
 {
     Plan plan {};
     const long long pairs = (long long) rows.max_count * group;
-    plan.tile_rows = pairs <= 16 ? 16 : 32;
+    plan.tile_rows = pairs <= 16 || (storage == WSP_F32 && head_width > 64) ? 16 : 32;
     plan.tiles = (int) ((pairs + plan.tile_rows - 1) / plan.tile_rows);
     plan.row_slots = (int) (pairs < plan.tile_rows ? pairs : plan.tile_rows);
     plan.slice = rows.sequences < kMostSequences ? rows.sequences : kMostSequences;
     const long long units = (long long) plan.tiles * heads * plan.slice;
     const size_t unit_floats = (size_t) plan.row_slots * (head_width + 2);
+    // As many splits as still run at once, or as keep the spans short.
     long long splits = (rows.max_length + kLeastSpan - 1) / kLeastSpan;
-    if (splits > kWantedBlocks / units)
-        splits = kWantedBlocks / units;
+    if (splits > kRoundBlocks / units)
+        splits = kRoundBlocks / units;
+    if (splits < (rows.max_length + kMostSpan - 1) / kMostSpan)
+        splits = (rows.max_length + kMostSpan - 1) / kMostSpan;
     if ((unsigned long long) splits > scratch_floats / unit_floats / units)
         splits = (long long) (scratch_floats / unit_floats / units);
     if (splits < 2)
