@@ -22,7 +22,7 @@ ARCH = "gfx950"
 
 DEVICE_SOURCES = ["ops.hip", "capi.hip", "cross_kv.hip", "fused_step.hip", "step_kernel.hip", "batch.hip",
                   "linear_product.hip", "split_product.hip", "attention_static.hip", "encoder.hip", "mel.hip", "paged.hip",
-                  "paged_attention.hip", "paged_capi.hip"]
+                  "paged_attention.hip", "paged_chunk.hip", "paged_capi.hip"]
 HOST_SOURCES = ["host/Gpu.cpp", "host/Net.cpp", "host/Half.cpp", "host/HipNet.cpp", "host/DecoderWeights.cpp",
                 "host/Decoder.cpp", "host/DecoderRecording.cpp", "host/Argmax.cpp", "host/GreedyDecoder.cpp", "host/BatchedDecoder.cpp",
                 "host/SafeTensors.cpp", "host/Tokenizer.cpp", "host/Encoder.cpp", "host/Whisper.cpp",
@@ -36,7 +36,7 @@ HOST_FLAGS = ["-O2", "-D__HIP_PLATFORM_AMD__", "-I" + os.path.join(ROCM, "includ
 # VGPRs (in AGPRs the compiler shuffles them between steps).
 SOURCE_FLAGS = {source: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for source in (
     "split_product.hip", "linear_product.hip", "mel.hip", "ops.hip",
-    "encoder.hip", "batch.hip", "paged_attention.hip")}
+    "encoder.hip", "batch.hip", "paged_attention.hip", "paged_chunk.hip")}
 
 
 def hipcc() -> str:

@@ -1,7 +1,7 @@
 // Attention over the pages of a cache (include/wsp_hip.h,
 // wsp_hip_paged_attention), on the matrix cores.
 #include "paged.h"
-#include "paged_device.h"
+#include "paged_attention.h"
 
 #include <algorithm>
 
@@ -9,78 +9,6 @@ namespace wsp::paged
 {
 namespace
 {
-// What a call asks, beside the cache and the rows.
-struct Query
-{
-    const float* q;
-    int q_stride;
-    int heads, group; // group: query heads a cached head serves
-    int causal;
-    float scale; // times log2(e): the softmax runs in powers of two
-    float* out;
-    int out_stride;
-};
-
-// How a call's keys are split: `splits` blocks of `span` keys each take a row
-// tile's keys, and their partial rows lie at [tile unit][split][row slot].
-struct Split
-{
-    int splits, span, row_slots;
-    float* partials;
-};
-
-// The rows one block computes: for one sequence and one cached head, `tile`
-// consecutive (new row, query head of the group) pairs, row-major.
-struct RowTile
-{
-    int first_row;   // the sequence's first packed row
-    int pairs;       // rows to compute times group
-    int past;        // position of the first new row (before 0: none)
-    int length;
-    int first, last; // this tile's pairs
-    int least, most; // keys that its first and its last row see
-    bool poisoned;   // the length passes max_length
-};
-
-__device__ __forceinline__ int keys_seen(const Query& query, const RowTile& t, int pair)
-{
-    const long long position = (long long) t.past + pair / query.group;
-    return position < 0 ? 0 : query.causal ? (int) position + 1 : t.length;
-}
-
-// False where the tile has no row.
-__device__ __forceinline__ bool find_tile(const Rows& rows, const Query& query, int sequence, int tile, int tile_rows,
-                                          RowTile& t)
-{
-    t.first_row = rows.starts[sequence];
-    const int end = rows.starts[sequence + 1];
-    if (t.first_row < 0 || end <= t.first_row)
-        return false;
-    const int count = end - t.first_row;
-    t.length = rows.lengths[sequence];
-    t.past = max(t.length, 0) - count;
-    t.pairs = min(min(count, rows.max_count), rows.rows - t.first_row) * query.group;
-    t.first = tile * tile_rows;
-    t.last = min(t.first + tile_rows, t.pairs) - 1;
-    if (t.last < t.first)
-        return false;
-    t.poisoned = t.length > rows.max_length;
-    t.least = keys_seen(query, t, t.first);
-    t.most = keys_seen(query, t, t.last);
-    return true;
-}
-
-// Blocks whose keys some row of the tile sees.
-__device__ __forceinline__ int splits_used(const RowTile& t, int span)
-{
-    return t.poisoned ? 1 : max(1, (t.most + span - 1) / span);
-}
-
-__device__ __forceinline__ float* partial_row(const Split& split, int unit, int which, int slot, int width)
-{
-    return split.partials + (((size_t) unit * split.splits + which) * split.row_slots + slot) * (width + 2);
-}
-
 // The largest over the four 16-lane groups, in each of their lanes.
 __device__ __forceinline__ float groups_max(float v)
 {
@@ -100,49 +28,6 @@ __device__ __forceinline__ float groups_sum(float v)
     const uint32_t half = __float_as_uint(v);
     const auto halves = __builtin_amdgcn_permlane32_swap(half, half, false, false);
     return __uint_as_float((uint32_t) halves[0]) + __uint_as_float((uint32_t) halves[1]);
-}
-
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32u __attribute__((aligned(1)));
-
-// Two E4M3 bytes (the low or high half of `packed`) as two fp16, exact.
-template <bool HIGH>
-__device__ __forceinline__ uint32_t e4m3_to_halves(uint32_t packed)
-{
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) packed, 1.f, HIGH));
-}
-
-// What the matrix cores multiply a storage as, and its bytes.
-template <int ST>
-constexpr int operand_of = ST == kE4M3 ? (int) kF16 : ST;
-template <int ST>
-constexpr int bytes_of = ST == kF32 ? 4 : ST == kE4M3 ? 1 : 2;
-
-// Two fp32 values as 16-bit parts packed in dwords: their sum is within 2^-22 of
-// each (two fp16 parts) or exact (three bf16 parts).
-template <int OT>
-__device__ __forceinline__ void cut_pair(float a, float b, uint32_t (&parts)[3])
-{
-    if constexpr (OT == kF16)
-    {
-        typedef _Float16 half2v __attribute__((ext_vector_type(2)));
-        const half2v high = {(_Float16) a, (_Float16) b};
-        const half2v low = {(_Float16) (a - (float) high[0]), (_Float16) (b - (float) high[1])};
-        parts[0] = __builtin_bit_cast(uint32_t, high);
-        parts[1] = __builtin_bit_cast(uint32_t, low);
-    }
-    else
-    {
-        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-#pragma unroll
-        for (int p = 0; p < 3; ++p)
-        {
-            const bf16x2 high = {(__bf16) a, (__bf16) b};
-            parts[p] = __builtin_bit_cast(uint32_t, high);
-            a -= (float) high[0];
-            b -= (float) high[1];
-        }
-    }
 }
 
 // ---------------------------------------------------------------------------
@@ -180,31 +65,6 @@ struct Tile // one lane's part of 32 keys and values, as stored
     uint32_t ke[2], ve[2];                       // E4M3: the exponents of rows 16b + 4g .. + 3
     bool bad[2];                                 // the page of keys 16b .. is none
 };
-
-template <int WORDS>
-__device__ __forceinline__ void load_words(const char* at, uint32_t (&words)[WORDS])
-{
-    if constexpr (WORDS == 1)
-        words[0] = *global(reinterpret_cast<const uint32_t*>(at));
-    else if constexpr (WORDS == 2)
-    {
-        const u32x2 v = *global(reinterpret_cast<const u32x2*>(at));
-        words[0] = v[0];
-        words[1] = v[1];
-    }
-    else
-    {
-        static_assert(WORDS % 4 == 0);
-#pragma unroll
-        for (int i = 0; i < WORDS / 4; ++i)
-        {
-            const u32x4 v = global(reinterpret_cast<const u32x4*>(at))[i];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                words[4 * i + j] = v[j];
-        }
-    }
-}
 
 // The pages of keys k0 .. k0 + 15 and k0 + 16 .. k0 + 31 (-1: none). k0 is below
 // `end`; of a sixteen that begins at or past it the first is named again (nothing
@@ -286,33 +146,14 @@ __device__ __forceinline__ uint32_t value_pair(const Tile<ST, W>& t, int b, int 
         return t.v[b][r][i];
 }
 
-// The bits of a dword's 16-bit halves that are finite, of type OT.
-template <int OT>
-__device__ __forceinline__ uint32_t finite_halves(uint32_t pair)
-{
-    constexpr uint32_t kTop = OT == kF16 ? 0x7C00u : 0x7F80u;
-    uint32_t kept = 0;
-    if ((pair & kTop) != kTop)
-        kept |= pair & 0xFFFFu;
-    if ((pair & (kTop << 16)) != kTop << 16)
-        kept |= pair & 0xFFFF0000u;
-    return kept;
-}
-
-// A stored value widened, E4M3 without its row's power.
-template <int ST>
-__device__ __forceinline__ float stored_value(const void* pool, size_t index)
-{
-    if constexpr (ST == kE4M3)
-        return __builtin_amdgcn_cvt_f32_fp8((int) static_cast<const uint8_t*>(pool)[index], 0);
-    else
-        return load1<ST>(pool, index);
-}
-
 constexpr int kTileWaves = 4;
 
+// Waves a SIMD the registers are kept to.
+template <int ST, int W, int QT>
+constexpr int kTileOccupancy = QT == 1 && W == 64 && ST != kF32 ? 3 : 2;
+
 template <int ST, int W, bool FULL, int QT>
-__global__ void __launch_bounds__(kTileWaves* kWave, 2) tile_attention_kernel(Cache cache, Rows rows, Query query,
+__global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)) tile_attention_kernel(Cache cache, Rows rows, Query query,
                                                                               Split split, int first_tile,
                                                                               int first_sequence)
 {
@@ -804,22 +645,28 @@ __global__ void __launch_bounds__(kJoinWaves* kWave) join_kernel(Cache cache, Ro
 
 constexpr int kMostBlocks = 65535; // of a launch's y and z extents
 
-template <int ST, int W, bool FULL, int QT>
-void launch_tiles(hipStream_t stream, const Cache& cache, const Rows& rows, const Query& query, const Plan& plan,
-                  const Split& split)
+void launch_tiles(hipStream_t stream, dim3 grid, int storage, const Cache& cache, const Rows& rows,
+                  const Query& query, const Split& split, int tile_rows, int first_tile, int first_sequence)
 {
-    for (int s = 0; s < rows.sequences; s += plan.slice)
-        for (int t = 0; t < plan.tiles; t += kMostBlocks)
-        {
-            const dim3 grid(split.splits * cache.heads, std::min(plan.tiles - t, kMostBlocks),
-                            std::min(rows.sequences - s, plan.slice));
-            tile_attention_kernel<ST, W, FULL, QT>
-                <<<grid, kTileWaves * kWave, 0, stream>>>(cache, rows, query, split, t, s);
-            if (split.splits > 1)
-                (split.splits <= kJoinWaves ? join_kernel<1> : join_kernel<8>)<<<
-                    dim3(cache.heads * split.row_slots, grid.y, grid.z), kJoinWaves * kWave, 0, stream>>>(
-                    cache, rows, query, split, 16 * QT, t, s);
-        }
+    by_storage(storage, [&](auto type) {
+        auto run = [&](auto width, auto full) {
+            if constexpr (width() == 64)
+                if (tile_rows == 32)
+                {
+                    tile_attention_kernel<type(), width(), full(), 2><<<grid, kTileWaves * kWave, 0, stream>>>(
+                        cache, rows, query, split, first_tile, first_sequence);
+                    return;
+                }
+            tile_attention_kernel<type(), width(), full(), 1>
+                <<<grid, kTileWaves * kWave, 0, stream>>>(cache, rows, query, split, first_tile, first_sequence);
+        };
+        using Narrow = std::integral_constant<int, 64>;
+        using Wide = std::integral_constant<int, 128>;
+        cache.head_width == 64    ? run(Narrow {}, std::true_type {})
+        : cache.head_width == 128 ? run(Wide {}, std::true_type {})
+        : cache.head_width < 64   ? run(Narrow {}, std::false_type {})
+                                  : run(Wide {}, std::false_type {});
+    });
 }
 } // namespace
 
@@ -833,22 +680,22 @@ hipError_t attention(hipStream_t stream, const wsp_paged_cache& cache, const wsp
     const Plan plan = plan_attention(rows, cache.storage, cache.heads, query.group, cache.head_width,
                                      scratch_bytes / sizeof(float));
     const Split split {plan.splits, plan.span, plan.row_slots, static_cast<float*>(scratch)};
-    by_storage(cache.storage, [&](auto storage) {
-        auto run = [&](auto width, auto full) {
-            if constexpr (storage() != kF32 || width() == 64)
-                if (plan.tile_rows == 32)
-                    return launch_tiles<storage(), width(), full(), 2>(stream, device_cache(cache), device_rows(rows),
-                                                                       query, plan, split);
-            launch_tiles<storage(), width(), full(), 1>(stream, device_cache(cache), device_rows(rows), query, plan,
-                                                        split);
-        };
-        using Narrow = std::integral_constant<int, 64>;
-        using Wide = std::integral_constant<int, 128>;
-        cache.head_width == 64    ? run(Narrow {}, std::true_type {})
-        : cache.head_width == 128 ? run(Wide {}, std::true_type {})
-        : cache.head_width < 64   ? run(Narrow {}, std::false_type {})
-                                  : run(Wide {}, std::false_type {});
-    });
+    const Cache pool = device_cache(cache);
+    const Rows packed = device_rows(rows);
+    for (int s = 0; s < rows.sequences; s += plan.slice)
+        for (int t = 0; t < plan.tiles; t += kMostBlocks)
+        {
+            const dim3 grid(split.splits * cache.heads, std::min(plan.tiles - t, kMostBlocks),
+                            std::min(rows.sequences - s, plan.slice));
+            if (plan.tile_rows == kChunkRows)
+                launch_chunks(stream, grid, cache.storage, pool, packed, query, split, t, s);
+            else
+                launch_tiles(stream, grid, cache.storage, pool, packed, query, split, plan.tile_rows, t, s);
+            if (split.splits > 1)
+                (split.splits <= kJoinWaves ? join_kernel<1> : join_kernel<8>)<<<
+                    dim3(cache.heads * split.row_slots, grid.y, grid.z), kJoinWaves * kWave, 0, stream>>>(
+                    pool, packed, query, split, plan.tile_rows, t, s);
+        }
     return hipGetLastError();
 }
 } // namespace wsp::paged

@@ -1,0 +1,571 @@
+// Attention of many rows over the pages of a cache of 16 or 8 bits: chunks of a
+// prompt (include/wsp_hip.h, wsp_hip_paged_attention).
+#include "paged_attention.h"
+
+namespace wsp::paged
+{
+namespace
+{
+typedef float float16v __attribute__((ext_vector_type(16)));
+
+// c + a·b over 16 k of 16-bit values of type OT, a 32 x 32 tile.
+template <int OT>
+__device__ __forceinline__ float16v mfma32(u32x4 a, u32x4 b, float16v c)
+{
+    if constexpr (OT == kF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0,
+                                                       0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                        0, 0, 0);
+}
+
+// The larger, and the sum, over the two halves of a wave.
+__device__ __forceinline__ float halves_max(float v)
+{
+    const uint32_t half = __float_as_uint(v);
+    const auto halves = __builtin_amdgcn_permlane32_swap(half, half, false, false);
+    return fmaxf(__uint_as_float((uint32_t) halves[0]), __uint_as_float((uint32_t) halves[1]));
+}
+__device__ __forceinline__ float halves_sum(float v)
+{
+    const uint32_t half = __float_as_uint(v);
+    const auto halves = __builtin_amdgcn_permlane32_swap(half, half, false, false);
+    return __uint_as_float((uint32_t) halves[0]) + __uint_as_float((uint32_t) halves[1]);
+}
+
+// A barrier for LDS alone: loads from memory stay in flight across it.
+__device__ __forceinline__ void lds_barrier()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: attention of a tile of 128 pairs (new row, head of the group), 32 a
+// wave, over keys [split·span, +span) of one cached head, 64 keys at a time
+// through LDS. The block converts and transposes what the storage holds once for
+// its 128 pairs: keys as [key][channel], values as [channel][key], 16-bit
+// operands of v_mfma_f32_32x32x16.
+//
+// S^T = K·Q^T leaves lane (n, h) with keys 8i + 4h + r (i, r < 4) of each 32 and
+// pair n. Its values 8s .. 8s + 7 (s < 2) are the operand of the s-th product over
+// 16 keys of O^T = V^T·P^T when that takes keys 4h .. 4h + 3 and 8 + 4h .. + 3 from
+// lane half h, so the transposed values keep those eight in one 16-byte run and
+// the weights cross no lanes.
+//
+// Queries and weights go in 16-bit parts, with the scalings of the kernel for few
+// rows. E4M3 rows' powers of two are multiplied into the 16-bit operands,
+// relative to the first key's: an E4M3 value times 2^-15 .. 2^7 is an fp16 value
+// exactly. A tile with a power outside that keeps its rows as they are and takes the
+// few rows' way: powers of keys multiply the scores, powers of values join them.
+//
+// Bound by the matrix cores (the two or three products a part) and, beside them,
+// the vector work of the softmax. While a tile is worked on the next is in flight
+// to registers; two blocks a CU fill each other's barriers.
+// ---------------------------------------------------------------------------
+constexpr int kChunkWaves = 4, kChunkKeys = 64;
+constexpr int kLeastShift = -15, kMostShift = 7;
+
+// The 16-byte run of run c of eight keys of a channel's row: eight consecutive
+// rows, and every fourth of 32, lie in different bank groups.
+__device__ __forceinline__ int value_slot(int row, int c)
+{
+    return 8 * row + (c ^ (row & 7) ^ (row >> 3 & 3));
+}
+
+template <int W>
+__device__ __forceinline__ int key_slot(int key, int c)
+{
+    return key * (W / 8) + (c ^ (key & 7));
+}
+
+// Eight E4M3 bytes times 2^power (as a float) as fp16.
+__device__ __forceinline__ u32x4 e4m3_run(uint32_t low, uint32_t high, float power)
+{
+    auto pair = [&](uint32_t packed, auto top) {
+        return __builtin_bit_cast(uint32_t,
+                                  __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) packed, power, decltype(top)::value));
+    };
+    return u32x4 {pair(low, std::false_type {}), pair(low, std::true_type {}), pair(high, std::false_type {}),
+                  pair(high, std::true_type {})};
+}
+
+template <int ST, int W, bool FULL>
+__global__ void __launch_bounds__(kChunkWaves* kWave, 2)
+    chunk_attention_kernel(Cache cache, Rows rows, Query query, Split split, int first_tile, int first_sequence)
+{
+    constexpr int OT = operand_of<ST>, kParts = parts_of<OT>();
+    constexpr float kBias = OT == kF16 ? 14.f : 0.f;
+    constexpr int kThreads = kChunkWaves * kWave;
+    constexpr int kKeyRuns = kChunkKeys * W / 8 / kThreads;      // runs of eight channels a thread loads
+    constexpr int kKeyWords = 2 * bytes_of<ST>;                  // dwords of one as stored
+    constexpr int kValueChannels = W / 32;                       // channels of eight keys a thread loads
+    constexpr int kValueWords = (kValueChannels * bytes_of<ST> + 3) / 4;
+    __shared__ u32x4 ks[kChunkKeys * W / 8];
+    __shared__ u32x4 vs[W * kChunkKeys / 8];
+    __shared__ __align__(16) float key_power[kChunkKeys], value_power[kChunkKeys], value_inverse[kChunkKeys];
+    // The last tile (its first key + 1) with a non-finite value that some pair sees,
+    // and the last E4M3 one whose rows' powers are not in the operands.
+    __shared__ int odd_tile, apart_tile;
+
+    const int which = blockIdx.x % split.splits, head = blockIdx.x / split.splits;
+    const int sequence = first_sequence + blockIdx.z;
+    const int tile = first_tile + (int) (gridDim.y - 1 - blockIdx.y); // (the tiles that see most come first)
+    RowTile tl;
+    if (!find_tile(rows, query, sequence, tile, kChunkRows, tl))
+        return;
+    const int used = splits_used(tl, split.span);
+    if (which >= used)
+        return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int lane = threadIdx.x % kWave, n = lane % 32, h = lane / 32;
+    const int width = FULL ? W : cache.head_width, row_bytes = width * bytes_of<ST>;
+    const int page_mask = (1 << cache.page_shift) - 1;
+    const int* table = rows.pages + (size_t) sequence * rows.table_width;
+    const int begin = which * split.span, end = tl.poisoned ? 0 : min(begin + split.span, tl.most);
+
+    // This wave's pairs: lane (n, h) holds channels 16j + 8h .. + 7 of pair n.
+    const int first = tl.first + 32 * wave, pair = first + n;
+    const bool real = pair <= tl.last;
+    const int seen = real ? min(keys_seen(query, tl, pair), end) : 0;
+    const int wave_least = first <= tl.last ? min(keys_seen(query, tl, first), end) : 0;
+    const int wave_most = first <= tl.last ? min(keys_seen(query, tl, min(first + 31, tl.last)), end) : 0;
+    u32x4 qp[W / 16][kParts];
+    float unit = 1.f; // the power of two that the parts leave out
+    {
+        const float* at = query.q + (size_t) (tl.first_row + (real ? pair : tl.first) / query.group) * query.q_stride
+                          + (size_t) (head * query.group + (real ? pair : tl.first) % query.group) * width;
+        float x[W / 16][8];
+        float top = 0.f;
+#pragma unroll
+        for (int j = 0; j < W / 16; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; i += 4)
+            {
+                float4v run = {0.f, 0.f, 0.f, 0.f};
+                if (real && (FULL || 16 * j + 8 * h < width))
+                    run = *reinterpret_cast<const float4u*>(at + 16 * j + 8 * h + i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                {
+                    x[j][i + e] = run[e] * query.scale;
+                    top = fmaxf(top, fabsf(x[j][i + e]));
+                }
+            }
+        int shift = 0;
+        if constexpr (OT == kF16)
+        {
+            // 2^13 <= top·2^shift < 2^14 (a pair of zeros, or not finite: as it is)
+            top = halves_max(top);
+            shift = top > 0.f && top < INFINITY ? min(140 - (int) (__float_as_uint(top) >> 23), 100) : 0;
+            unit = ldexpf(1.f, -shift);
+        }
+#pragma unroll
+        for (int j = 0; j < W / 16; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+            {
+                uint32_t cut[3];
+                if constexpr (OT == kF16)
+                    cut_pair<OT>(ldexpf(x[j][2 * i], shift), ldexpf(x[j][2 * i + 1], shift), cut);
+                else
+                    cut_pair<OT>(x[j][2 * i], x[j][2 * i + 1], cut);
+#pragma unroll
+                for (int p = 0; p < kParts; ++p)
+                    qp[j][p][i] = cut[p];
+            }
+    }
+
+    // What a thread loads of a tile: key runs threadIdx.x + 256·i (run key_run of key
+    // key_of + kKeysAtOnce·i), and of the eight keys of run `value_run` (16·wave +
+    // 4h .. + 3 and 8 more on) the channels from value_channel on.
+    constexpr int kKeysAtOnce = kThreads / (W / 8); // 16 or 32
+    const int key_run = threadIdx.x % (W / 8), key_of = threadIdx.x / (W / 8);
+    const int value_channel = threadIdx.x % 32 * kValueChannels, value_run = 2 * wave + h;
+    const bool key_real = FULL || 8 * key_run < width;
+    const uint32_t key_offset = key_of % 16 * row_bytes + 8 * key_run * bytes_of<ST>;
+    const uint32_t value_offset = 4 * h * row_bytes + (FULL || value_channel < width ? value_channel : 0) * bytes_of<ST>;
+    struct Raw
+    {
+        uint32_t k[kKeyRuns][kKeyWords];
+        uint32_t v[8][kValueWords];
+        uint32_t ke[ST == kE4M3 ? kKeyRuns : 1], ve[2]; // the exponents of those rows
+    } raw;
+    typedef int int4v __attribute__((ext_vector_type(4)));
+    static_assert(kChunkKeys == 64, "four sixteens");
+    int4v pages; // of each sixteen of the tile in flight (-1: none)
+
+    auto load = [&](int k0) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+            pages[s] = k0 + 16 * s < end ? page_of(table, rows.table_width, cache.page_shift, cache.pages, k0 + 16 * s)
+                                         : -1;
+        // (Pages are the same for a whole wave, so these addresses are scalars.)
+        auto row_of = [&](int page, int key) {
+            return pool_row(max(page, 0), head, key & page_mask, cache.heads, cache.page_shift);
+        };
+#pragma unroll
+        for (int i = 0; i < kKeyRuns; ++i)
+        {
+            const bool second = kKeysAtOnce == 32 && wave >= 2; // of the 32 keys of one i
+            const int page = kKeysAtOnce == 16 ? pages[i] : i == 0 ? (second ? pages[1] : pages[0])
+                                                                   : (second ? pages[3] : pages[2]);
+            const size_t row = row_of(page, k0 + kKeysAtOnce * i + (second ? 16 : 0));
+            if (key_real)
+                load_words(static_cast<const char*>(cache.keys) + row * row_bytes + key_offset, raw.k[i]);
+            else
+#pragma unroll
+                for (int j = 0; j < kKeyWords; ++j)
+                    raw.k[i][j] = 0;
+            if constexpr (ST == kE4M3)
+                raw.ke[i] = *global(cache.key_exponents + row + (uint32_t) (key_of % 16));
+        }
+        const int page = wave == 0 ? pages[0] : wave == 1 ? pages[1] : wave == 2 ? pages[2] : pages[3];
+        const size_t row = row_of(page, k0 + 16 * wave);
+        const char* values = static_cast<const char*>(cache.values) + row * row_bytes;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+        {
+            const char* at = values + (8 * (i / 4) + i % 4) * row_bytes + value_offset;
+            if constexpr (kValueChannels * bytes_of<ST> == 2)
+                raw.v[i][0] = *global(reinterpret_cast<const uint16_t*>(at));
+            else
+                load_words(at, raw.v[i]);
+        }
+        if constexpr (ST == kE4M3)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                raw.ve[i] = *(const __attribute__((address_space(1))) u32u*) (cache.value_exponents + row + 8 * i
+                                                                             + (uint32_t) (4 * h));
+    };
+
+    // E4M3: the powers that the operands leave out, those of the block's first rows.
+    int key_base = kExponentBias, value_base = kExponentBias;
+    if (ST == kE4M3 && begin < end)
+    {
+        const int page = page_of(table, rows.table_width, cache.page_shift, cache.pages, begin);
+        const size_t row = pool_row(max(page, 0), head, begin & page_mask, cache.heads, cache.page_shift);
+        key_base = cache.key_exponents[row];
+        value_base = cache.value_exponents[row];
+    }
+    // 2^(byte - base) as a float's bits, for bytes within a float's range of the base.
+    auto power_bits = [](uint32_t byte, int base) { return (byte + (uint32_t) (kExponentBias - base)) << 23; };
+    auto value_byte = [&](int i) { return raw.ve[i / 4] >> (8 * (i % 4)) & 255u; };
+    auto key_of_value = [&](int i) { return 16 * wave + 8 * (i / 4) + 4 * h + i % 4; };
+
+    // Before the barrier behind which the tile goes to LDS: whether its rows' powers
+    // do not all fit the operands.
+    auto look = [&](int k0) {
+        if constexpr (ST == kE4M3)
+        {
+            bool fits = true;
+#pragma unroll
+            for (int i = 0; i < kKeyRuns; ++i)
+                fits = fits
+                       && ((unsigned) ((int) raw.ke[i] - key_base - kLeastShift) <= (unsigned) (kMostShift - kLeastShift)
+                           || k0 + key_of + kKeysAtOnce * i >= end);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                fits = fits
+                       && ((unsigned) ((int) value_byte(i) - value_base - kLeastShift)
+                               <= (unsigned) (kMostShift - kLeastShift)
+                           || k0 + key_of_value(i) >= end);
+            if (!fits)
+                apart_tile = k0 + 1;
+        }
+    };
+
+    // The raw tile to LDS.
+    auto stage = [&](int k0, bool apart) {
+        if (ST == kE4M3 && apart)
+        {
+            if (key_run == 0)
+#pragma unroll
+                for (int i = 0; i < kKeyRuns; ++i)
+                    key_power[key_of + kKeysAtOnce * i] = ldexpf(1.f, (int) raw.ke[i] - key_base);
+            if (threadIdx.x % 32 == 0)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                {
+                    const int key = key_of_value(i), power = (int) value_byte(i) - value_base;
+                    value_power[key] = (float) power;
+                    value_inverse[key] = k0 + key < end ? ldexpf(1.f, -power) : 0.f;
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < kKeyRuns; ++i)
+        {
+            u32x4 run;
+            if constexpr (ST == kE4M3)
+                run = e4m3_run(raw.k[i][0], raw.k[i][1],
+                               apart ? 1.f : __uint_as_float(power_bits(raw.ke[i], key_base)));
+            else
+                run = u32x4 {raw.k[i][0], raw.k[i][1], raw.k[i][2], raw.k[i][3]};
+            ks[key_slot<W>(key_of + kKeysAtOnce * i, key_run)] = run;
+        }
+        // Values as pairs of channels, then pairs of keys of one channel.
+        uint32_t pairs[8][kValueChannels / 2];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+        {
+            const float power = ST == kE4M3 && !apart ? __uint_as_float(power_bits(value_byte(i), value_base)) : 1.f;
+#pragma unroll
+            for (int c = 0; c < kValueChannels / 2; ++c)
+                if constexpr (ST == kE4M3)
+                    pairs[i][c] = __builtin_bit_cast(
+                        uint32_t, c == 0 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) raw.v[i][0], power, false)
+                                         : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) raw.v[i][0], power, true));
+                else
+                    pairs[i][c] = raw.v[i][c];
+        }
+        // A weight of zero hides a value only while it is finite: values that no pair
+        // sees count as zero, and non-finite ones among keys that some pairs see are
+        // added behind the products, to those pairs alone.
+        const int page = wave == 0 ? pages[0] : wave == 1 ? pages[1] : wave == 2 ? pages[2] : pages[3];
+        if (k0 + kChunkKeys > min(tl.least, end) || page < 0)
+        {
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+            {
+                const bool unseen = k0 + key_of_value(i) >= end || page < 0;
+#pragma unroll
+                for (int c = 0; c < kValueChannels / 2; ++c)
+                {
+                    const uint32_t kept = unseen ? 0u : finite_halves<OT>(pairs[i][c]);
+                    odd = odd || (!unseen && kept != pairs[i][c]);
+                    pairs[i][c] = kept;
+                }
+            }
+            if (odd)
+                odd_tile = k0 + 1;
+        }
+#pragma unroll
+        for (int c = 0; c < kValueChannels; c += 2)
+        {
+            u32x4 low, high;
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+            {
+                low[d] = __builtin_amdgcn_perm(pairs[2 * d + 1][c / 2], pairs[2 * d][c / 2], 0x05040100);
+                high[d] = __builtin_amdgcn_perm(pairs[2 * d + 1][c / 2], pairs[2 * d][c / 2], 0x07060302);
+            }
+            vs[value_slot(value_channel + c, value_run)] = low;
+            vs[value_slot(value_channel + c + 1, value_run)] = high;
+        }
+    };
+
+    float16v o[W / 32];
+#pragma unroll
+    for (int c = 0; c < W / 32; ++c)
+        o[c] = float16v {};
+    float m = -INFINITY, l = 0.f;
+    if (threadIdx.x == 0)
+        odd_tile = apart_tile = 0;
+    __syncthreads();
+
+    if (begin < end)
+        load(begin);
+    for (int k0 = begin; k0 < end; k0 += kChunkKeys)
+    {
+        look(k0);
+        lds_barrier(); // (the tile before is read)
+        const bool apart = ST == kE4M3 && apart_tile == k0 + 1;
+        stage(k0, apart);
+        const int4v tile_pages = pages; // (the next tile's take their place)
+        const float known = ST == kE4M3 ? ldexpf(unit, key_base - kExponentBias) : unit;
+        lds_barrier();
+        if (k0 + kChunkKeys < end)
+            load(k0 + kChunkKeys);
+        if (k0 >= wave_most) // (none of this wave's pairs sees a key)
+            continue;
+
+        const bool odd = odd_tile == k0 + 1;
+        // 32 keys at a time: what is live fits the registers of two blocks a CU.
+#pragma unroll 1
+        for (int b = 0; b < 2; ++b)
+        {
+            const int from = k0 + 32 * b;
+            if (from >= wave_most)
+                break;
+            float16v s = {};
+            u32x4 key[W / 16];
+#pragma unroll
+            for (int j = 0; j < W / 16; ++j)
+                key[j] = ks[key_slot<W>(32 * b + n, 2 * j + h)];
+#pragma unroll
+            for (int j = 0; j < W / 16; ++j)
+#pragma unroll
+                for (int p = kParts - 1; p >= 0; --p)
+                    s = mfma32<OT>(key[j], qp[j][p], s);
+            // Value 4i + r of s is key 8i + 4h + r of the 32. Scores in powers of two, but
+            // for `scale`, which the multiply-add before the powers takes in.
+            float scale = ST == kE4M3 ? known : unit;
+            if (ST == kE4M3 && apart)
+            {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                {
+                    const float4v kp = *reinterpret_cast<const float4v*>(&key_power[32 * b + 8 * i + 4 * h]);
+                    const float4v vp = *reinterpret_cast<const float4v*>(&value_power[32 * b + 8 * i + 4 * h]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        s[4 * i + r] = __builtin_fmaf(s[4 * i + r], known * kp[r], vp[r]);
+                }
+                scale = 1.f;
+            }
+            const bool first_bad = (b == 0 ? tile_pages[0] : tile_pages[2]) < 0;
+            const bool second_bad = (b == 0 ? tile_pages[1] : tile_pages[3]) < 0 && from + 16 < end;
+            if (from + 32 > wave_least || first_bad || second_bad)
+            {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                {
+                    if (i < 8 ? first_bad : second_bad)
+                        s[i] = __builtin_nanf("");
+                    s[i] = from + 8 * (i / 4) + 4 * h + i % 4 < seen ? s[i] : -INFINITY;
+                }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                top = fmaxf(top, s[i]);
+            // The maximum is rounded up to a whole power of two: what it rescales stays exact.
+            const float m_new = fmaxf(m, ceilf(halves_max(top) * scale));
+            const float finite = m_new == -INFINITY ? 0.f : m_new, base = finite - kBias;
+            if (__any(m_new != m))
+            {
+                const float alpha = __builtin_amdgcn_exp2f(m - finite);
+                l *= alpha;
+#pragma unroll
+                for (int c = 0; c < W / 32; ++c)
+                    o[c] *= alpha;
+                m = m_new;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale, -base));
+            float own[4] = {0.f, 0.f, 0.f, 0.f};
+            if (ST == kE4M3 && apart)
+            {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                {
+                    const float4v inverse = *reinterpret_cast<const float4v*>(&value_inverse[32 * b + 8 * i + 4 * h]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        own[r] += s[4 * i + r] * inverse[r];
+                }
+            }
+            else
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    own[i % 4] += s[i];
+            l += (own[0] + own[1]) + (own[2] + own[3]);
+            u32x4 weights[2][kParts];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                {
+                    uint32_t cut[3];
+                    cut_pair<OT>(s[8 * t + 2 * i], s[8 * t + 2 * i + 1], cut);
+#pragma unroll
+                    for (int p = 0; p < kParts; ++p)
+                        weights[t][p][i] = cut[p];
+                }
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+            {
+                u32x4 value[W / 32];
+#pragma unroll
+                for (int c = 0; c < W / 32; ++c)
+                    value[c] = vs[value_slot(32 * c + n, 4 * b + 2 * t + h)];
+#pragma unroll
+                for (int p = kParts - 1; p >= 0; --p)
+#pragma unroll
+                    for (int c = 0; c < W / 32; ++c)
+                        o[c] = mfma32<OT>(value[c], weights[t][p], o[c]);
+            }
+            if (odd) // (rare: infinities or NaN among the new rows' values)
+#pragma unroll 1
+                for (int key = 0; key < 32; ++key)
+                {
+                    // Key 16t + 8i + 4h + r is value 4i + r of lane half h's weights t. (Only
+                    // that a weight is not zero matters: the first part of it does.)
+                    uint32_t held = 0;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (8 * (key / 16) + 4 * (key / 8 % 2) + key % 4 == 8 * t + i)
+                                held = i % 2 == 0 ? weights[t][0][i / 2] << 16 : weights[t][0][i / 2] & 0xFFFF0000u;
+                    const float weight = __uint_as_float(__shfl(held, n + 32 * (key / 4 % 2)));
+                    const int position = from + key;
+                    const int page = page_of(table, rows.table_width, cache.page_shift, cache.pages, position);
+                    if (position >= seen || page < 0)
+                        continue;
+                    const size_t row = pool_row(page, head, position & page_mask, cache.heads, cache.page_shift);
+#pragma unroll
+                    for (int c = 0; c < W / 32; ++c)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                        {
+                            const int channel = 32 * c + 8 * (i / 4) + 4 * h + i % 4;
+                            const float value =
+                                channel < width ? stored_value<ST>(cache.values, row * width + channel) : 0.f;
+                            if (!isfinite(value))
+                                o[c][i] += weight * value;
+                        }
+                }
+        }
+    }
+
+    // o[c][4i + r] is channel 32c + 8i + 4h + r of pair n; times the values' power.
+    l = halves_sum(l);
+    if (tl.poisoned)
+        l = __builtin_nanf("");
+    if (!real)
+        return;
+    const float power = ldexpf(1.f, value_base - kExponentBias);
+    const float by = used > 1 ? power : l == 0.f ? 0.f : power / l;
+    const int unit_index = ((int) blockIdx.z * (int) gridDim.y + (int) blockIdx.y) * cache.heads + head;
+    float* part = partial_row(split, unit_index, which, 32 * wave + n, width);
+    float* out = used > 1 ? part + 2
+                          : query.out + (size_t) (tl.first_row + pair / query.group) * query.out_stride
+                                + (size_t) (head * query.group + pair % query.group) * width;
+    if (used > 1 && h == 0)
+    {
+        part[0] = m;
+        part[1] = l;
+    }
+#pragma unroll
+    for (int c = 0; c < W / 32; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (FULL || 32 * c + 8 * i + 4 * h < width)
+                *reinterpret_cast<float4u*>(out + 32 * c + 8 * i + 4 * h) =
+                    float4v {o[c][4 * i], o[c][4 * i + 1], o[c][4 * i + 2], o[c][4 * i + 3]} * by;
+}
+} // namespace
+
+void launch_chunks(hipStream_t stream, dim3 grid, int storage, const Cache& cache, const Rows& rows,
+                   const Query& query, const Split& split, int first_tile, int first_sequence)
+{
+    by_storage(storage, [&](auto type) {
+        auto run = [&](auto width, auto full) {
+            if constexpr (type() != kF32)
+                chunk_attention_kernel<type(), width(), full()><<<grid, kChunkWaves * kWave, 0, stream>>>(
+                    cache, rows, query, split, first_tile, first_sequence);
+        };
+        using Narrow = std::integral_constant<int, 64>;
+        using Wide = std::integral_constant<int, 128>;
+        cache.head_width == 64    ? run(Narrow {}, std::true_type {})
+        : cache.head_width == 128 ? run(Wide {}, std::true_type {})
+        : cache.head_width < 64   ? run(Narrow {}, std::false_type {})
+                                  : run(Wide {}, std::false_type {});
+    });
+}
+} // namespace wsp::paged

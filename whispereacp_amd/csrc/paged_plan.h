@@ -91,6 +91,7 @@ struct Plan
     int slice;
 };
 
+constexpr int kChunkRows = 128;   // of the kernel for many rows
 constexpr int kRoundBlocks = 768; // blocks that run at once, three a CU
 constexpr int kLeastSpan = 256;   // two turns of a block's waves
 constexpr int kMostSpan = 2048;   // lengths differ: blocks of longer spans end apart
@@ -101,7 +102,10 @@ inline Plan plan_attention(const wsp_paged_rows& rows, int storage, int heads, i
 {
     Plan plan {};
     const long long pairs = (long long) rows.max_count * group;
-    plan.tile_rows = pairs <= 16 || (storage == WSP_F32 && head_width > 64) ? 16 : 32;
+    if (storage == WSP_F32)
+        plan.tile_rows = pairs <= 16 || head_width > 64 ? 16 : 32;
+    else
+        plan.tile_rows = pairs <= 16 ? 16 : pairs <= 32 && head_width <= 64 ? 32 : kChunkRows;
     plan.tiles = (int) ((pairs + plan.tile_rows - 1) / plan.tile_rows);
     plan.row_slots = (int) (pairs < plan.tile_rows ? pairs : plan.tile_rows);
     plan.slice = rows.sequences < kMostSequences ? rows.sequences : kMostSequences;
@@ -118,7 +122,7 @@ inline Plan plan_attention(const wsp_paged_rows& rows, int storage, int heads, i
     if (splits < 2)
         splits = 1;
     plan.span = (int) ((rows.max_length + splits - 1) / splits);
-    plan.span = plan.span < kLeastSpan ? kLeastSpan : (plan.span + 31) / 32 * 32;
+    plan.span = plan.span < kLeastSpan ? kLeastSpan : (plan.span + 63) / 64 * 64;
     plan.splits = rows.max_length <= plan.span ? 1 : (rows.max_length + plan.span - 1) / plan.span;
     return plan;
 }
