@@ -103,10 +103,13 @@ __device__ __forceinline__ void cut_pair(float a, float b, uint32_t (&parts)[3])
     {
         typedef _Float16 half2v __attribute__((ext_vector_type(2)));
         uint32_t packed = __builtin_bit_cast(uint32_t, half2v {(_Float16) a, (_Float16) b});
-        asm("" : "+v"(packed)); // (the differences are taken from the pair, not rounded anew)
+        // (Opaque, so that each difference is one multiply-add that reads its half of the
+        // pair, not a rounding anew, a widening and a subtraction.)
+        float minus = -1.f;
+        asm("" : "+v"(packed), "+s"(minus));
         const half2v high = __builtin_bit_cast(half2v, packed);
-        const half2v low = {(_Float16) __builtin_fmaf((float) high[0], -1.f, a),
-                            (_Float16) __builtin_fmaf((float) high[1], -1.f, b)};
+        const half2v low = {(_Float16) __builtin_fmaf((float) high[0], minus, a),
+                            (_Float16) __builtin_fmaf((float) high[1], minus, b)};
         parts[0] = packed;
         parts[1] = __builtin_bit_cast(uint32_t, low);
     }

@@ -83,13 +83,20 @@ __device__ __forceinline__ Pages find_pages(const Cache& cache, const int* table
              page_of(table, table_width, cache.page_shift, cache.pages, second_key(k0, end))}};
 }
 
-// Keys and values k0 .. k0 + 31 of a cached head.
+// Where a lane's parts of a key and of a value row lie in a sixteen's rows, in bytes.
+struct Offsets
+{
+    uint32_t key, value;
+};
+
+// Keys and values k0 .. k0 + 31 of a cached head. (The pages are the same for the
+// wave: what is not in `at` is scalar.)
 template <int ST, int W, bool FULL>
-__device__ __forceinline__ void load_tile(const Cache& cache, const Pages& pages, int head, int k0, int end,
+__device__ __forceinline__ void load_tile(const Cache& cache, const Pages& pages, int head, int k0, int end, Offsets at,
                                           Tile<ST, W>& t)
 {
-    const int lane = threadIdx.x % kWave, li = lane % 16, g = lane / 16;
-    const int mask = (1 << cache.page_shift) - 1, row_bytes = cache.head_width * bytes_of<ST>;
+    const int g = threadIdx.x % kWave / 16;
+    const int mask = (1 << cache.page_shift) - 1, row_bytes = (FULL ? W : cache.head_width) * bytes_of<ST>;
 #pragma unroll
     for (int b = 0; b < 2; ++b)
     {
@@ -104,20 +111,18 @@ __device__ __forceinline__ void load_tile(const Cache& cache, const Pages& pages
         {
             uint32_t run[4] = {0, 0, 0, 0};
             if (FULL || 16 * (4 * i + g) < row_bytes)
-                load_words(keys + li * row_bytes + 16 * (4 * i + g), run);
+                load_words(keys + 64 * i + at.key, run);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 t.k[b][4 * i + j] = run[j];
         }
-        // (Lanes past the row read its start: they hold channels nobody stores.)
-        const int channel = FULL || li * (W / 16) < cache.head_width ? li * (W / 16) : 0;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-            load_words(values + (4 * g + r) * row_bytes + channel * bytes_of<ST>, t.v[b][r]);
+            load_words(values + r * row_bytes + at.value, t.v[b][r]);
         if constexpr (ST == kE4M3)
         {
-            t.ke[b] = *(const __attribute__((address_space(1))) u32u*) (cache.key_exponents + row + 4 * g);
-            t.ve[b] = *(const __attribute__((address_space(1))) u32u*) (cache.value_exponents + row + 4 * g);
+            t.ke[b] = *(const __attribute__((address_space(1))) u32u*) (cache.key_exponents + row + (uint32_t) (4 * g));
+            t.ve[b] = *(const __attribute__((address_space(1))) u32u*) (cache.value_exponents + row + (uint32_t) (4 * g));
         }
     }
 }
@@ -173,7 +178,7 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
         return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int lane = threadIdx.x % kWave, li = lane % 16, g = lane / 16;
-    const int width = cache.head_width;
+    const int width = FULL ? W : cache.head_width;
     const int* table = rows.pages + (size_t) sequence * rows.table_width;
     const int begin = which * split.span, end = tl.poisoned ? 0 : min(begin + split.span, tl.most);
 
@@ -252,7 +257,6 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
         // Keys that not every pair sees, or whose page is none, take the careful way.
         const bool careful = k0 + kKeys > min(tl.least, end) || kv.bad[0] || kv.bad[1];
         uint32_t weights[QT][OT == kF32 ? 1 : kParts][OT == kF32 ? 8 : 4];
-        float alpha[QT];
 #pragma unroll
         for (int t = 0; t < QT; ++t)
         {
@@ -274,22 +278,18 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
                 }
                 else
                 {
-                    float4v part[kParts];
+                    s[b] = float4v {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int j = 0; j < W / 32; ++j)
                     {
                         const u32x4 key = key_operand<ST, W>(kv, b, j);
 #pragma unroll
-                        for (int p = 0; p < kParts; ++p)
-                            part[p] = mfma16<OT>(key,
-                                                 u32x4 {qp[t][p][4 * j], qp[t][p][4 * j + 1], qp[t][p][4 * j + 2],
-                                                        qp[t][p][4 * j + 3]},
-                                                 j == 0 ? float4v {0.f, 0.f, 0.f, 0.f} : part[p]);
+                        for (int p = kParts - 1; p >= 0; --p)
+                            s[b] = mfma16<OT>(key,
+                                              u32x4 {qp[t][p][4 * j], qp[t][p][4 * j + 1], qp[t][p][4 * j + 2],
+                                                     qp[t][p][4 * j + 3]},
+                                              s[b]);
                     }
-                    s[b] = part[kParts - 1];
-#pragma unroll
-                    for (int p = kParts - 2; p >= 0; --p)
-                        s[b] += part[p];
                 }
             }
             // Scores in powers of two; E4M3 ones with the value rows' powers in them.
@@ -334,8 +334,15 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
             // score, zero in its place: the weights are zero.)
             const float m_new = fmaxf(m[t], ceilf(groups_max(top)));
             const float finite = m_new == -INFINITY ? 0.f : m_new, base = finite - kBias;
-            alpha[t] = __builtin_amdgcn_exp2f(m[t] - finite);
-            m[t] = m_new;
+            if (__any(m_new != m[t])) // (seldom, but for the first keys)
+            {
+                const float alpha = __builtin_amdgcn_exp2f(m[t] - finite);
+                l[t] *= alpha;
+#pragma unroll
+                for (int c = 0; c < CPL; ++c)
+                    o[t][c] *= alpha;
+                m[t] = m_new;
+            }
             float own = 0.f;
 #pragma unroll
             for (int b = 0; b < 2; ++b)
@@ -345,7 +352,7 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
                     s[b][r] = __builtin_amdgcn_exp2f(s[b][r] - base);
                     own += ST == kE4M3 ? s[b][r] * inverse[b][r] : s[b][r];
                 }
-            l[t] = l[t] * alpha[t] + own;
+            l[t] += own;
 #pragma unroll
             for (int i = 0; i < (OT == kF32 ? 8 : 4); ++i)
                 if constexpr (OT == kF32)
@@ -360,10 +367,8 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
                 }
         }
 
-        // The rows, two channels of each lane's at a time. Every 32 keys are summed
-        // on their own and join the row by the multiply-add that rescales it.
+        // The rows, two channels of each lane's at a time.
         bool odd = false;
-        const float4v none = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < CPL; c += 2)
         {
@@ -396,12 +401,10 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
                     {
-                        float4v part = none;
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
-                            part = __builtin_amdgcn_mfma_f32_16x16x4f32(v[e][i], __uint_as_float(weights[t][0][i]),
-                                                                        part, 0, 0, 0);
-                        o[t][c + e] = o[t][c + e] * alpha[t] + part;
+                            o[t][c + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                v[e][i], __uint_as_float(weights[t][0][i]), o[t][c + e], 0, 0, 0);
                     }
             }
             else
@@ -434,32 +437,39 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
                     {
-                        float4v part = none;
 #pragma unroll
                         for (int p = kParts - 1; p >= 0; --p)
-                            part = mfma16<OT>(v[e],
-                                              u32x4 {weights[t][p][0], weights[t][p][1], weights[t][p][2],
-                                                     weights[t][p][3]},
-                                              part);
-                        o[t][c + e] = o[t][c + e] * alpha[t] + part;
+                            o[t][c + e] = mfma16<OT>(v[e],
+                                                     u32x4 {weights[t][p][0], weights[t][p][1], weights[t][p][2],
+                                                            weights[t][p][3]},
+                                                     o[t][c + e]);
                     }
             }
         }
         if (careful && __any(odd)) // (rare: infinities or NaN among the new rows' values)
 #pragma unroll
             for (int t = 0; t < QT; ++t)
+            {
+                constexpr int kDwords = OT == kF32 ? 8 : 4;
+                uint32_t parts[kDwords]; // (opaque: nothing of this is worked out before it is needed)
+#pragma unroll
+                for (int i = 0; i < kDwords; ++i)
+                {
+                    parts[i] = weights[t][0][i];
+                    asm("" : "+v"(parts[i]));
+                }
 #pragma unroll 1
                 for (int key = 0; key < kKeys; ++key)
                 {
                     // Key 16b + 4g + r is held by lane group g. (Only that its weight is
                     // not zero matters: the first part of it does.)
-                    const int at = 4 * (key / 16) + key % 4;
-                    uint32_t pair = 0;
+                    uint32_t held = 0;
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        if (i == at)
-                            pair = weights[t][0][OT == kF32 ? i : i / 2];
-                    const uint32_t held = OT == kF32 ? pair : at % 2 == 0 ? pair << 16 : pair & 0xFFFF0000u;
+                        if (4 * (key / 16) + key % 4 == i)
+                            held = OT == kF32   ? parts[i * kDwords / 8]
+                                   : i % 2 == 0 ? parts[i * kDwords / 8] << 16
+                                                : parts[i * kDwords / 8] & 0xFFFF0000u;
                     const float weight = __uint_as_float(__shfl(held, li + 16 * (key / 4 % 4)));
                     const int position = k0 + key;
                     const int page = page_of(table, rows.table_width, cache.page_shift, cache.pages, position);
@@ -479,6 +489,7 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
                                 o[t][c][r] += weight * value;
                         }
                 }
+            }
     };
 
     // The next keys are in flight while these are worked on (not where two tiles
@@ -488,9 +499,12 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
     int k0 = begin + kKeys * wave;
     if (k0 < end)
     {
+        // (Value lanes past the row read its start: they hold channels nobody stores.)
+        const int row_bytes = width * bytes_of<ST>, channel = FULL || li * CPL < width ? li * CPL : 0;
+        const Offsets at {(uint32_t) (li * row_bytes + 16 * g), (uint32_t) (4 * g * row_bytes + channel * bytes_of<ST>)};
         Tile<ST, W> now;
         Pages pages = find_pages(cache, table, rows.table_width, k0, end);
-        load_tile<ST, W, FULL>(cache, pages, head, k0, end, now);
+        load_tile<ST, W, FULL>(cache, pages, head, k0, end, at, now);
         if (k0 + kStride < end)
             pages = find_pages(cache, table, rows.table_width, k0 + kStride, end);
         for (; k0 + kStride < end; k0 += kStride)
@@ -498,7 +512,7 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
             if constexpr (!kAhead)
                 work(now, k0);
             Tile<ST, W> next;
-            load_tile<ST, W, FULL>(cache, pages, head, k0 + kStride, end, next);
+            load_tile<ST, W, FULL>(cache, pages, head, k0 + kStride, end, at, next);
             if (k0 + 2 * kStride < end)
                 pages = find_pages(cache, table, rows.table_width, k0 + 2 * kStride, end);
             if constexpr (kAhead)

@@ -255,23 +255,58 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, 2)
     auto value_byte = [&](int i) { return raw.ve[i / 4] >> (8 * (i % 4)) & 255u; };
     auto key_of_value = [&](int i) { return 16 * wave + 8 * (i / 4) + 4 * h + i % 4; };
 
+    auto bad_pages = [&](int k0) { // a bit for each sixteen of the tile in flight
+        int bad = 0;
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+            bad |= pages[s] < 0 && k0 + 16 * s < end ? 1 << s : 0;
+        return bad;
+    };
+
     // Before the barrier behind which the tile goes to LDS: whether its rows' powers
     // do not all fit the operands.
     auto look = [&](int k0) {
         if constexpr (ST == kE4M3)
         {
-            bool fits = true;
+            int key_bytes[kKeyRuns], value_bytes[8];
 #pragma unroll
             for (int i = 0; i < kKeyRuns; ++i)
-                fits = fits
-                       && ((unsigned) ((int) raw.ke[i] - key_base - kLeastShift) <= (unsigned) (kMostShift - kLeastShift)
-                           || k0 + key_of + kKeysAtOnce * i >= end);
+                key_bytes[i] = (int) raw.ke[i];
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                fits = fits
-                       && ((unsigned) ((int) value_byte(i) - value_base - kLeastShift)
-                               <= (unsigned) (kMostShift - kLeastShift)
-                           || k0 + key_of_value(i) >= end);
+                value_bytes[i] = (int) value_byte(i);
+            if (k0 + kChunkKeys > end || bad_pages(k0) != 0)
+            {
+                // Rows that no pair sees may hold anything.
+                const int bad = bad_pages(k0);
+#pragma unroll
+                for (int i = 0; i < kKeyRuns; ++i)
+                {
+                    const int key = key_of + kKeysAtOnce * i;
+                    if (k0 + key >= end || (bad >> (key / 16) & 1) != 0)
+                        key_bytes[i] = key_base;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (k0 + key_of_value(i) >= end || (bad >> wave & 1) != 0)
+                        value_bytes[i] = value_base;
+            }
+            int low = key_bytes[0], high = key_bytes[0];
+#pragma unroll
+            for (int i = 1; i < kKeyRuns; ++i)
+            {
+                low = min(low, key_bytes[i]);
+                high = max(high, key_bytes[i]);
+            }
+            bool fits = low - key_base >= kLeastShift && high - key_base <= kMostShift;
+            low = high = value_bytes[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i)
+            {
+                low = min(low, value_bytes[i]);
+                high = max(high, value_bytes[i]);
+            }
+            fits = fits && low - value_base >= kLeastShift && high - value_base <= kMostShift;
             if (!fits)
                 apart_tile = k0 + 1;
         }
@@ -374,7 +409,7 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, 2)
         lds_barrier(); // (the tile before is read)
         const bool apart = ST == kE4M3 && apart_tile == k0 + 1;
         stage(k0, apart);
-        const int4v tile_pages = pages; // (the next tile's take their place)
+        const int bad = bad_pages(k0); // (the next tile's take their place)
         const float known = ST == kE4M3 ? ldexpf(unit, key_base - kExponentBias) : unit;
         lds_barrier();
         if (k0 + kChunkKeys < end)
@@ -390,6 +425,7 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, 2)
             const int from = k0 + 32 * b;
             if (from >= wave_most)
                 break;
+            __builtin_amdgcn_s_setprio(1);
             float16v s = {};
             u32x4 key[W / 16];
 #pragma unroll
@@ -400,6 +436,7 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, 2)
 #pragma unroll
                 for (int p = kParts - 1; p >= 0; --p)
                     s = mfma32<OT>(key[j], qp[j][p], s);
+            __builtin_amdgcn_s_setprio(0);
             // Value 4i + r of s is key 8i + 4h + r of the 32. Scores in powers of two, but
             // for `scale`, which the multiply-add before the powers takes in.
             float scale = ST == kE4M3 ? known : unit;
@@ -416,8 +453,7 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, 2)
                 }
                 scale = 1.f;
             }
-            const bool first_bad = (b == 0 ? tile_pages[0] : tile_pages[2]) < 0;
-            const bool second_bad = (b == 0 ? tile_pages[1] : tile_pages[3]) < 0 && from + 16 < end;
+            const bool first_bad = (bad >> (2 * b) & 1) != 0, second_bad = (bad >> (2 * b + 1) & 1) != 0;
             if (from + 32 > wave_least || first_bad || second_bad)
             {
 #pragma unroll
@@ -476,6 +512,7 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, 2)
                     for (int p = 0; p < kParts; ++p)
                         weights[t][p][i] = cut[p];
                 }
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int t = 0; t < 2; ++t)
             {
@@ -489,7 +526,16 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, 2)
                     for (int c = 0; c < W / 32; ++c)
                         o[c] = mfma32<OT>(value[c], weights[t][p], o[c]);
             }
+            __builtin_amdgcn_s_setprio(0);
             if (odd) // (rare: infinities or NaN among the new rows' values)
+            {
+                uint32_t parts[8]; // (opaque: nothing of this is worked out before it is needed)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                {
+                    parts[i] = weights[i / 4][0][i % 4];
+                    asm("" : "+v"(parts[i]));
+                }
 #pragma unroll 1
                 for (int key = 0; key < 32; ++key)
                 {
@@ -497,11 +543,9 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, 2)
                     // that a weight is not zero matters: the first part of it does.)
                     uint32_t held = 0;
 #pragma unroll
-                    for (int t = 0; t < 2; ++t)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (8 * (key / 16) + 4 * (key / 8 % 2) + key % 4 == 8 * t + i)
-                                held = i % 2 == 0 ? weights[t][0][i / 2] << 16 : weights[t][0][i / 2] & 0xFFFF0000u;
+                    for (int i = 0; i < 16; ++i)
+                        if (8 * (key / 16) + 4 * (key / 8 % 2) + key % 4 == i)
+                            held = i % 2 == 0 ? parts[i / 2] << 16 : parts[i / 2] & 0xFFFF0000u;
                     const float weight = __uint_as_float(__shfl(held, n + 32 * (key / 4 % 2)));
                     const int position = from + key;
                     const int page = page_of(table, rows.table_width, cache.page_shift, cache.pages, position);
@@ -520,6 +564,7 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, 2)
                                 o[c][i] += weight * value;
                         }
                 }
+            }
         }
     }
 
