@@ -8,7 +8,7 @@ namespace wsp::paged
 {
 namespace
 {
-constexpr int kBlock = 256;
+constexpr int kBlock = 256, kWavesPerBlock = kBlock / kWave;
 constexpr int kMinExponent = -80, kMaxExponent = 120;
 
 // The power of two of an E4M3 row: the least k in range with amax <= 448·2^k
@@ -88,10 +88,14 @@ __device__ __forceinline__ void store_stored4(void* pool, size_t index, const fl
 }
 
 // ---------------------------------------------------------------------------
-// Append and read: LANES lanes (16 for heads up to 64 wide, 32 for wider ones)
-// a (row, head), four values of its key and of its value each. Append takes the
-// row's largest magnitude over those lanes, so a row is read once.
+// Append and read: a wave a packed row, LANES lanes (16 for heads up to 64 wide, 32
+// for wider ones) a head, four values of its key and of its value each, and kTurns
+// heads one after the other, all their loads in flight at once. The row's sequence,
+// position and page are the same for the wave, so the search and the addresses are
+// scalar. Append takes a head's largest magnitude over its lanes: a row is read once.
 // ---------------------------------------------------------------------------
+constexpr int kTurns = 4;
+
 template <int LANES>
 __device__ __forceinline__ float lanes_max(float v)
 {
@@ -101,55 +105,86 @@ __device__ __forceinline__ float lanes_max(float v)
     return v;
 }
 
+// Where a packed row lies: its page (-1: none) and its place there.
+struct Place
+{
+    int sequence, page, place;
+    bool before; // its position is before its sequence
+};
+
+__device__ __forceinline__ Place place_of(const Cache& cache, const Rows& rows, int row)
+{
+    Place at {-1, -1, 0, false};
+    if (row >= rows.rows)
+        return at;
+    at.sequence = sequence_of(rows.starts, rows.sequences, row);
+    if (at.sequence < 0)
+        return at;
+    const long long position = position_of(rows.starts, rows.lengths, at.sequence, row);
+    at.before = position < 0;
+    if (!at.before)
+    {
+        at.page = page_at(cache, rows, at.sequence, (int) position);
+        at.place = (int) position & ((1 << cache.page_shift) - 1);
+    }
+    return at;
+}
+
 template <int ST, int LANES>
 __global__ void __launch_bounds__(kBlock) append_kernel(Cache cache, Rows rows, const float* __restrict__ keys,
                                                         int key_stride, const float* __restrict__ values,
                                                         int value_stride)
 {
-    const long long unit = ((long long) blockIdx.x * kBlock + threadIdx.x) / LANES;
-    const int row = (int) (unit / cache.heads), head = (int) (unit % cache.heads);
-    const int c = 4 * (threadIdx.x % LANES);
-    if (row >= rows.rows) // (whole groups of lanes leave together)
+    const int row = blockIdx.x * kWavesPerBlock + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const Place at = place_of(cache, rows, row);
+    if (at.page < 0)
         return;
-    const int sequence = sequence_of(rows.starts, rows.sequences, row);
-    if (sequence < 0)
-        return;
-    const long long position = position_of(rows.starts, rows.lengths, sequence, row);
-    const int page = position < 0 ? -1 : page_at(cache, rows, sequence, (int) position);
-    if (page < 0)
-        return;
-    const bool inside = c < cache.head_width;
-    float4v k = {0.f, 0.f, 0.f, 0.f}, v = k;
-    if (inside)
-    {
-        k = *reinterpret_cast<const float4u*>(keys + (size_t) row * key_stride + (size_t) head * cache.head_width + c);
-        v = *reinterpret_cast<const float4u*>(values + (size_t) row * value_stride + (size_t) head * cache.head_width
-                                              + c);
-    }
-    const size_t slot = pool_row(page, head, (int) position & ((1 << cache.page_shift) - 1), cache.heads,
-                                 cache.page_shift);
-    int key_exponent = 0, value_exponent = 0;
-    if constexpr (ST == kE4M3)
-    {
-        float key_max = 0.f, value_max = 0.f;
+    constexpr int kHeads = kWave / LANES; // a turn
+    const int first = blockIdx.y * kHeads * kTurns + threadIdx.x % kWave / LANES, c = 4 * (threadIdx.x % LANES);
+    const int width = cache.head_width;
+    const bool inside = c < width;
+    const float* const key_row = keys + (size_t) row * key_stride;
+    const float* const value_row = values + (size_t) row * value_stride;
+    float4v k[kTurns], v[kTurns];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < kTurns; ++i)
+    {
+        const int head = first + kHeads * i;
+        k[i] = v[i] = float4v {0.f, 0.f, 0.f, 0.f};
+        if (inside && head < cache.heads)
         {
-            key_max = fmaxf(key_max, finite_magnitude(k[i]));
-            value_max = fmaxf(value_max, finite_magnitude(v[i]));
-        }
-        key_exponent = row_exponent(lanes_max<LANES>(key_max));
-        value_exponent = row_exponent(lanes_max<LANES>(value_max));
-        if (c == 0)
-        {
-            cache.key_exponents[slot] = (uint8_t) (key_exponent + kExponentBias);
-            cache.value_exponents[slot] = (uint8_t) (value_exponent + kExponentBias);
+            k[i] = *reinterpret_cast<const float4u*>(key_row + (size_t) head * width + c);
+            v[i] = *reinterpret_cast<const float4u*>(value_row + (size_t) head * width + c);
         }
     }
-    if (inside)
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i)
     {
-        store_stored4<ST>(cache.keys, slot * cache.head_width + c, k, key_exponent);
-        store_stored4<ST>(cache.values, slot * cache.head_width + c, v, value_exponent);
+        const int head = first + kHeads * i;
+        const size_t slot = pool_row(at.page, head, at.place, cache.heads, cache.page_shift);
+        int key_exponent = 0, value_exponent = 0;
+        if constexpr (ST == kE4M3)
+        {
+            float key_max = 0.f, value_max = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+            {
+                key_max = fmaxf(key_max, finite_magnitude(k[i][e]));
+                value_max = fmaxf(value_max, finite_magnitude(v[i][e]));
+            }
+            key_exponent = row_exponent(lanes_max<LANES>(key_max));
+            value_exponent = row_exponent(lanes_max<LANES>(value_max));
+            if (c == 0 && head < cache.heads)
+            {
+                cache.key_exponents[slot] = (uint8_t) (key_exponent + kExponentBias);
+                cache.value_exponents[slot] = (uint8_t) (value_exponent + kExponentBias);
+            }
+        }
+        if (inside && head < cache.heads)
+        {
+            store_stored4<ST>(cache.keys, slot * width + c, k[i], key_exponent);
+            store_stored4<ST>(cache.values, slot * width + c, v[i], value_exponent);
+        }
     }
 }
 
@@ -157,66 +192,78 @@ template <int ST, int LANES>
 __global__ void __launch_bounds__(kBlock) read_kernel(Cache cache, Rows rows, float* __restrict__ keys,
                                                       int key_stride, float* __restrict__ values, int value_stride)
 {
-    const long long unit = ((long long) blockIdx.x * kBlock + threadIdx.x) / LANES;
-    const int row = (int) (unit / cache.heads), head = (int) (unit % cache.heads);
-    const int c = 4 * (threadIdx.x % LANES);
-    if (row >= rows.rows || c >= cache.head_width)
+    const int row = blockIdx.x * kWavesPerBlock + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const Place at = place_of(cache, rows, row);
+    if (at.sequence < 0)
         return;
-    const int sequence = sequence_of(rows.starts, rows.sequences, row);
-    if (sequence < 0)
+    constexpr int kHeads = kWave / LANES; // a turn
+    const int first = blockIdx.y * kHeads * kTurns + threadIdx.x % kWave / LANES, c = 4 * (threadIdx.x % LANES);
+    const int width = cache.head_width;
+    if (c >= width)
         return;
-    const long long position = position_of(rows.starts, rows.lengths, sequence, row);
-    float4v k = {0.f, 0.f, 0.f, 0.f}, v = k;
-    if (position >= 0)
+    float4v k[kTurns], v[kTurns];
+    int key_exponents[kTurns], value_exponents[kTurns];
+    const float other = at.before ? 0.f : __builtin_nanf(""); // where there is no page
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i)
     {
-        const int page = page_at(cache, rows, sequence, (int) position);
-        if (page < 0)
-            k = v = float4v {0.f, 0.f, 0.f, 0.f} + __builtin_nanf("");
-        else
+        const int head = first + kHeads * i;
+        k[i] = v[i] = float4v {other, other, other, other};
+        key_exponents[i] = value_exponents[i] = kExponentBias;
+        if (at.page >= 0 && head < cache.heads)
         {
-            const size_t slot = pool_row(page, head, (int) position & ((1 << cache.page_shift) - 1), cache.heads,
-                                         cache.page_shift);
-            k = load_stored4<ST>(cache.keys, slot * cache.head_width + c);
-            v = load_stored4<ST>(cache.values, slot * cache.head_width + c);
+            const size_t slot = pool_row(at.page, head, at.place, cache.heads, cache.page_shift);
+            k[i] = load_stored4<ST>(cache.keys, slot * width + c);
+            v[i] = load_stored4<ST>(cache.values, slot * width + c);
             if constexpr (ST == kE4M3)
             {
-                const int key_exponent = (int) cache.key_exponents[slot] - kExponentBias;
-                const int value_exponent = (int) cache.value_exponents[slot] - kExponentBias;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                {
-                    k[i] = ldexpf(k[i], key_exponent);
-                    v[i] = ldexpf(v[i], value_exponent);
-                }
+                key_exponents[i] = cache.key_exponents[slot];
+                value_exponents[i] = cache.value_exponents[slot];
             }
         }
     }
-    *reinterpret_cast<float4u*>(keys + (size_t) row * key_stride + (size_t) head * cache.head_width + c) = k;
-    *reinterpret_cast<float4u*>(values + (size_t) row * value_stride + (size_t) head * cache.head_width + c) = v;
+    float* const key_row = keys + (size_t) row * key_stride;
+    float* const value_row = values + (size_t) row * value_stride;
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i)
+    {
+        const int head = first + kHeads * i;
+        if (head >= cache.heads)
+            return;
+        if constexpr (ST == kE4M3)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+            {
+                k[i][e] = ldexpf(k[i][e], key_exponents[i] - kExponentBias);
+                v[i][e] = ldexpf(v[i][e], value_exponents[i] - kExponentBias);
+            }
+        *reinterpret_cast<float4u*>(key_row + (size_t) head * width + c) = k[i];
+        *reinterpret_cast<float4u*>(value_row + (size_t) head * width + c) = v[i];
+    }
 }
 
-// The same with the storage and the lanes of a (row, head).
+// f called with the storage and the lanes of a head as compile-time constants, and
+// the grid: rows, and the heads that a wave does not take.
 template <class F>
-void by_lanes(const wsp_paged_cache& cache, F&& f)
+void by_lanes(const wsp_paged_cache& cache, const wsp_paged_rows& rows, F&& f)
 {
     by_storage(cache.storage, [&](auto storage) {
-        cache.head_width <= 64 ? f(storage, std::integral_constant<int, 16> {})
-                               : f(storage, std::integral_constant<int, 32> {});
+        auto run = [&](auto lanes) {
+            constexpr int kHeads = kTurns * kWave / decltype(lanes)::value;
+            f(storage, lanes,
+              dim3((unsigned) (((long long) rows.rows + kWavesPerBlock - 1) / kWavesPerBlock),
+                   (cache.heads + kHeads - 1) / kHeads));
+        };
+        cache.head_width <= 64 ? run(std::integral_constant<int, 16> {}) : run(std::integral_constant<int, 32> {});
     });
-}
-
-unsigned row_blocks(const wsp_paged_cache& cache, const wsp_paged_rows& rows)
-{
-    const long long threads = (long long) rows.rows * cache.heads * (cache.head_width <= 64 ? 16 : 32);
-    return (unsigned) ((threads + kBlock - 1) / kBlock);
 }
 } // namespace
 
 hipError_t append(hipStream_t stream, const wsp_paged_cache& cache, const wsp_paged_rows& rows, const float* keys,
                   int key_stride, const float* values, int value_stride)
 {
-    by_lanes(cache, [&](auto storage, auto lanes) {
-        append_kernel<storage(), lanes()><<<row_blocks(cache, rows), kBlock, 0, stream>>>(
+    by_lanes(cache, rows, [&](auto storage, auto lanes, dim3 grid) {
+        append_kernel<storage(), lanes()><<<grid, kBlock, 0, stream>>>(
             device_cache(cache), device_rows(rows), keys, key_stride, values, value_stride);
     });
     return hipGetLastError();
@@ -225,8 +272,8 @@ hipError_t append(hipStream_t stream, const wsp_paged_cache& cache, const wsp_pa
 hipError_t read(hipStream_t stream, const wsp_paged_cache& cache, const wsp_paged_rows& rows, float* keys,
                 int key_stride, float* values, int value_stride)
 {
-    by_lanes(cache, [&](auto storage, auto lanes) {
-        read_kernel<storage(), lanes()><<<row_blocks(cache, rows), kBlock, 0, stream>>>(
+    by_lanes(cache, rows, [&](auto storage, auto lanes, dim3 grid) {
+        read_kernel<storage(), lanes()><<<grid, kBlock, 0, stream>>>(
             device_cache(cache), device_rows(rows), keys, key_stride, values, value_stride);
     });
     return hipGetLastError();

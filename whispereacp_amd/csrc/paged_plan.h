@@ -92,6 +92,7 @@ struct Plan
 };
 
 constexpr int kChunkRows = 128;   // of the kernel for many rows
+constexpr int kChunkBlocks = 384;
 constexpr int kRoundBlocks = 768; // blocks that run at once, three a CU
 constexpr int kLeastSpan = 256;   // two turns of a block's waves
 constexpr int kMostSpan = 2048;   // lengths differ: blocks of longer spans end apart
@@ -102,10 +103,15 @@ inline Plan plan_attention(const wsp_paged_rows& rows, int storage, int heads, i
 {
     Plan plan {};
     const long long pairs = (long long) rows.max_count * group;
-    if (storage == WSP_F32)
-        plan.tile_rows = pairs <= 16 || head_width > 64 ? 16 : 32;
+    // Blocks of 128 rows where they make a round and a half of the chip: each takes
+    // longer (16 sequences of 512 rows over 2048 keys of 12 heads of 64, fp16: 128 us and 176
+    // in blocks of 32; 4 sequences 87 and 55; 64 of 32 rows over 4096, heads of 128 in
+    // E4M3, 237 and 147 in blocks of 16).
+    const long long chunks = (pairs + kChunkRows - 1) / kChunkRows * heads * rows.sequences;
+    if (storage != WSP_F32 && pairs > kChunkRows / 2 && chunks >= kChunkBlocks)
+        plan.tile_rows = kChunkRows;
     else
-        plan.tile_rows = pairs <= 16 ? 16 : pairs <= 32 && head_width <= 64 ? 32 : kChunkRows;
+        plan.tile_rows = pairs <= 16 || head_width > 64 ? 16 : 32;
     plan.tiles = (int) ((pairs + plan.tile_rows - 1) / plan.tile_rows);
     plan.row_slots = (int) (pairs < plan.tile_rows ? pairs : plan.tile_rows);
     plan.slice = rows.sequences < kMostSequences ? rows.sequences : kMostSequences;

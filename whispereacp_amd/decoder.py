@@ -103,8 +103,7 @@ class KernelContext:
     def paged_append(self, cache, rows, keys, values):
         """Stores the packed rows keys and values [rows.rows, heads·head_width] in
         their sequences' pages (paged.PagedCache, paged.PagedRows)."""
-        cache.check(self.device)
-        rows.check(self.device)
+        rows.check(cache, self.device)
         width = cache.heads * cache.head_width
         self._check(self.lib.wsp_hip_paged_append(
             self.handle, cache.table, rows.table, ptr(keys), rows.stride(keys, width, self.device), ptr(values),
@@ -112,8 +111,7 @@ class KernelContext:
 
     def paged_read(self, cache, rows, keys, values):
         """Writes the packed rows' stored values to keys and values, fp32."""
-        cache.check(self.device)
-        rows.check(self.device)
+        rows.check(cache, self.device)
         width = cache.heads * cache.head_width
         self._check(self.lib.wsp_hip_paged_read(
             self.handle, cache.table, rows.table, ptr(keys), rows.stride(keys, width, self.device), ptr(values),
@@ -122,8 +120,7 @@ class KernelContext:
     def paged_attention(self, cache, rows, q, heads, causal, scale, out):
         """Attention of the packed rows q [rows.rows, heads·head_width] over their
         sequences' pages, into out."""
-        cache.check(self.device)
-        rows.check(self.device)
+        rows.check(cache, self.device)
         width = heads * cache.head_width
         self._check(self.lib.wsp_hip_paged_attention(
             self.handle, cache.table, rows.table, ptr(q), rows.stride(q, width, self.device), heads, int(causal), scale,

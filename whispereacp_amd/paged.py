@@ -29,9 +29,7 @@ STORAGES = {"F32": (N.WSP_F32, torch.float32), "F16": (N.WSP_F16, torch.float16)
 _CODES = {dtype: code for code, dtype in STORAGES.values()}
 
 
-def _on(tensor: torch.Tensor, device: int) -> None:
-    if not tensor.is_cuda or tensor.get_device() != device:
-        raise ValueError(f"a tensor on {tensor.device} for a context on device {device}")
+_FLOAT = torch.float32
 
 
 class PagedCache:
@@ -58,6 +56,7 @@ class PagedCache:
             raise ValueError("the pool's tensors lie on one device")
         self.keys, self.values, self.key_exponents, self.value_exponents = keys, values, key_exponents, value_exponents
         self.pages, self.heads, self.page_rows, self.head_width = keys.shape
+        self.device = keys.get_device()  # -1: not a GPU's
         self._ctable = N.wsp_paged_cache(_CODES[keys.dtype], self.pages, self.page_rows, self.heads, self.head_width,
                                          keys.data_ptr(), values.data_ptr(),
                                          *(t.data_ptr() for t in exponents or ()))
@@ -75,9 +74,6 @@ class PagedCache:
         exponents = [torch.empty(shape[:3], dtype=torch.uint8, device=f"cuda:{device}")
                      for _ in range(2 if storage == "E4M3" else 0)]
         return cls(*pools, *exponents)
-
-    def check(self, device: int) -> None:
-        _on(self.keys, device)
 
 
 class PagedRows:
@@ -98,17 +94,20 @@ class PagedRows:
         if len({t.device for t in self._keep}) != 1:
             raise ValueError("starts, lengths and the table lie on one device")
         self.rows = rows
+        self.device = lengths.get_device()
         self._ctable = N.wsp_paged_rows(sequences, rows, max_count, max_length, table.shape[1], starts.data_ptr(),
                                         lengths.data_ptr(), table.data_ptr())
         self.table = ctypes.byref(self._ctable)
 
-    def check(self, device: int) -> None:
-        _on(self._keep[0], device)
+    def check(self, cache: PagedCache, device: int) -> None:
+        if cache.device != device or self.device != device:
+            raise ValueError(f"a pool on device {cache.device} and rows on {self.device} for a context on device {device}")
 
     def stride(self, tensor: torch.Tensor, width: int, device: int) -> int:
         """How far the packed rows of `tensor` lie apart."""
-        if tensor.dtype != torch.float32 or tensor.dim() != 2 or tensor.shape[0] < self.rows \
-                or tensor.shape[1] != width or (tensor.stride(1) != 1 and width > 1):
+        shape, strides = tensor.shape, tensor.stride()
+        if tensor.dtype is not _FLOAT or len(shape) != 2 or shape[0] < self.rows or shape[1] != width or strides[1] != 1:
             raise ValueError(f"packed rows are fp32 [{self.rows}, {width}], each row in one run")
-        _on(tensor, device)
-        return tensor.stride(0) if tensor.shape[0] > 1 else max(width, tensor.stride(0))
+        if tensor.get_device() != device:
+            raise ValueError(f"a tensor on {tensor.device} for a context on device {device}")
+        return strides[0] if shape[0] > 1 else max(width, strides[0])
