@@ -3,6 +3,7 @@
 // fused_step.hip. No call here allocates after wsp_hip_ctx_create.
 #include "capi_internal.h"
 #include "ops.h"
+#include "paged_plan.h"
 
 #include <algorithm>
 #include <cstdarg>
@@ -90,24 +91,30 @@ int wsp_hip_ctx_create(const wsp_decoder_shape* shape, int device, void* stream,
         // three parts).
         ctx->parts_bytes = std::max<size_t>(
             16 << 20, wsp::ops::parts_bytes((size_t) longest * std::max(shape->width, shape->feed_forward_width)));
-        // One block: the attention workspace, the argmax candidates, the parts.
+        // One block: the attention workspace, the argmax candidates, the paged
+        // attention's counters, the parts.
         auto rounded = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
         const size_t attention = rounded(std::max(ctx->attention_floats, wsp::ops::kQueryAttentionFloats)
                                          * sizeof(float));
         const size_t candidates = rounded(ctx->argmax_candidates * sizeof(float));
+        const size_t counters = rounded(wsp::paged::kSplitUnits * sizeof(unsigned int));
         char* block = nullptr;
-        status = hip_status(ctx, hipMalloc(&block, attention + 2 * candidates + ctx->parts_bytes), "workspace");
+        status = hip_status(ctx, hipMalloc(&block, attention + 2 * candidates + counters + ctx->parts_bytes),
+                            "workspace");
         if (status == WSP_OK)
         {
             ctx->attention_workspace = reinterpret_cast<float*>(block);
             ctx->argmax_values = reinterpret_cast<float*>(block + attention);
             ctx->argmax_indices = reinterpret_cast<uint32_t*>(block + attention + candidates);
-            ctx->parts = block + attention + 2 * candidates;
+            ctx->paged_counters = reinterpret_cast<unsigned int*>(block + attention + 2 * candidates);
+            ctx->parts = block + attention + 2 * candidates + counters;
             // The prompt attention's per-head counters start at zero (each launch
             // leaves them zero again).
             status = hip_status(ctx, hipMemset(ctx->attention_workspace, 0,
                                                wsp::ops::kAttentionCounters * sizeof(unsigned int)),
                                 "attention workspace");
+            if (status == WSP_OK) // (the same of the paged attention's)
+                status = hip_status(ctx, hipMemset(ctx->paged_counters, 0, counters), "paged attention");
         }
     }
     if (status == WSP_OK)

@@ -26,6 +26,8 @@ struct wsp_hip_ctx
     void* parts = nullptr;
     size_t parts_bytes = 0;
 
+    unsigned int* paged_counters = nullptr; // paged::kSplitUnits, zero between calls
+
     void* fused = nullptr; // fused-step state (fused_step.hip)
 
     // wsp_hip_step_report_next: the host pair the next sampling step writes

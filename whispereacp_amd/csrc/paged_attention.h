@@ -19,11 +19,13 @@ struct Query
 };
 
 // How a call's keys are split: `splits` blocks of `span` keys each take a row
-// tile's keys, and their partial rows lie at [tile unit][split][row slot].
+// tile's keys, their partial rows lie at [tile unit][split][row slot], and a unit's
+// counter tells its last block (zero between launches; null: another launch joins).
 struct Split
 {
     int splits, span, row_slots;
     float* partials;
+    unsigned int* counters;
 };
 
 // The rows one block computes: for one sequence and one cached head, `tile`
@@ -71,6 +73,12 @@ __device__ __forceinline__ bool find_tile(const Rows& rows, const Query& query, 
 __device__ __forceinline__ int splits_used(const RowTile& t, int span)
 {
     return t.poisoned ? 1 : max(1, (t.most + span - 1) / span);
+}
+
+__device__ __forceinline__ float* out_of(const RowTile& t, const Query& query, int head, int pair, int width, int c)
+{
+    return query.out + (size_t) (t.first_row + pair / query.group) * query.out_stride
+           + (size_t) (head * query.group + pair % query.group) * width + c;
 }
 
 __device__ __forceinline__ float* partial_row(const Split& split, int unit, int which, int slot, int width)
@@ -176,8 +184,7 @@ __device__ __forceinline__ void load_words(const char* at, uint32_t (&words)[WOR
 }
 
 // One launch over row tiles first_tile on and sequences first_sequence on (its
-// grid: splits·heads, tiles, sequences), by the kernel for many rows
-// (paged_chunk.hip).
+// grid: heads, tiles, sequences), by the kernel for many rows (paged_chunk.hip).
 void launch_chunks(hipStream_t stream, dim3 grid, int storage, const Cache& cache, const Rows& rows,
-                   const Query& query, const Split& split, int first_tile, int first_sequence);
+                   const Query& query, int first_tile, int first_sequence);
 } // namespace wsp::paged

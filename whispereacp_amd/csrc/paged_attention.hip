@@ -153,6 +153,16 @@ __device__ __forceinline__ uint32_t value_pair(const Tile<ST, W>& t, int b, int 
 
 constexpr int kTileWaves = 4;
 
+// A float that blocks of one launch hand to each other.
+__device__ __forceinline__ void store_shared(float* at, float value)
+{
+    __hip_atomic_store(at, value, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float load_shared(const float* at)
+{
+    return __hip_atomic_load(const_cast<float*>(at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 // Waves a SIMD the registers are kept to.
 template <int ST, int W, int QT>
 constexpr int kTileOccupancy = QT == 1 && W == 64 && ST != kF32 ? 3 : 2;
@@ -168,6 +178,7 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
     __shared__ float sums[kWaves][16][W];
 
     const int which = blockIdx.x % split.splits, head = blockIdx.x / split.splits;
+    const int unit = ((int) blockIdx.z * (int) gridDim.y + (int) blockIdx.y) * cache.heads + head;
     const int sequence = first_sequence + blockIdx.z;
     const int tile = first_tile + (int) (gridDim.y - 1 - blockIdx.y); // (the tiles that see most come first)
     RowTile tl;
@@ -184,7 +195,7 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
 
     // The queries: lane (li, g) holds the channels of pair li that it holds of a key.
     uint32_t qp[QT][OT == kF32 ? 1 : kParts][OT == kF32 ? W / 4 : W / 8];
-    float unit[QT]; // the power of two that the parts leave out
+    float left[QT]; // the power of two that the parts leave out
     int seen[QT];
 #pragma unroll
     for (int t = 0; t < QT; ++t)
@@ -207,7 +218,7 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
             for (int j = 0; j < 4; ++j)
                 x[i + j] = run[j] * query.scale;
         }
-        unit[t] = 1.f;
+        left[t] = 1.f;
         if constexpr (OT == kF32)
 #pragma unroll
             for (int i = 0; i < W / 4; ++i)
@@ -227,7 +238,7 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
 #pragma unroll
                 for (int i = 0; i < W / 4; ++i)
                     x[i] = ldexpf(x[i], shift);
-                unit[t] = ldexpf(1.f, -shift);
+                left[t] = ldexpf(1.f, -shift);
             }
 #pragma unroll
             for (int i = 0; i < W / 8; ++i)
@@ -302,12 +313,12 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
                     if constexpr (ST == kE4M3)
                     {
                         const uint32_t ke = kv.ke[b] >> (8 * r) & 255u, ve = kv.ve[b] >> (8 * r) & 255u;
-                        s[b][r] = __builtin_fmaf(s[b][r], unit[t] * __uint_as_float(ke << 23),
+                        s[b][r] = __builtin_fmaf(s[b][r], left[t] * __uint_as_float(ke << 23),
                                                  (float) ve - (float) kExponentBias);
                         inverse[b][r] = __uint_as_float((254u - ve) << 23);
                     }
                     else if constexpr (OT == kF16)
-                        s[b][r] *= unit[t];
+                        s[b][r] *= left[t];
                 }
             if (careful)
             {
@@ -566,30 +577,99 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
             if (tl.poisoned)
                 numerator = denominator = __builtin_nanf("");
             if (used == 1)
-                query.out[(size_t) (tl.first_row + pair / query.group) * query.out_stride
-                          + (size_t) (head * query.group + pair % query.group) * width + c] =
-                    denominator == 0.f ? 0.f : numerator / denominator;
+                *out_of(tl, query, head, pair, width, c) = denominator == 0.f ? 0.f : numerator / denominator;
             else
             {
-                const int unit_index = ((int) blockIdx.z * (int) gridDim.y + (int) blockIdx.y) * cache.heads + head;
-                float* part = partial_row(split, unit_index, which, 16 * t + at, width);
-                part[2 + c] = numerator;
+                float* part = partial_row(split, unit, which, 16 * t + at, width);
+                store_shared(part + 2 + c, numerator);
                 if (c == 0)
                 {
-                    part[0] = largest;
-                    part[1] = denominator;
+                    store_shared(part, largest);
+                    store_shared(part + 1, denominator);
                 }
             }
         }
     }
+    if (used == 1 || split.counters == nullptr)
+        return;
+
+    // Few splits: the last block of a row tile to come here joins its splits, in their order. The
+    // partial rows pass between blocks by device-scope accesses, which no cache of one
+    // chiplet keeps: each wave waits until its own are done, the barrier until every
+    // wave's are, and only then the count goes up. (Fences instead, which write back and
+    // drop the whole cache for each block, made a step of 64 long sequences 728 us.)
+    __shared__ int joins;
+    wait_loads<0>();
+    __syncthreads();
+    if (threadIdx.x == 0)
+        joins = __hip_atomic_fetch_add(&split.counters[unit], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+                == (unsigned) (used - 1);
+    __syncthreads();
+    if (!joins)
+        return;
+    // First what each split's row of a pair is multiplied by (a row is a wave's at a
+    // time), then the rows.
+    static_assert(sizeof(sums) >= kJoinRows * sizeof(float), "a factor for each partial row");
+    float* const factors = &sums[0][0][0]; // [row slot][split]
+    const int slots = tl.last - tl.first + 1;
+    for (int slot = wave; slot < slots; slot += kWaves)
+    {
+        const float* first = partial_row(split, unit, 0, slot, width);
+        const size_t pitch = (size_t) split.row_slots * (width + 2);
+        float largest = -INFINITY;
+        for (int i = lane; i < used; i += kWave)
+        {
+            const float top = load_shared(first + i * pitch);
+            factors[slot * used + i] = top;
+            largest = fmaxf(largest, top);
+        }
+        largest = wave_max(largest);
+        float total = 0.f;
+        for (int i = lane; i < used; i += kWave)
+        {
+            const float part = load_shared(first + i * pitch + 1);
+            const float factor = part == 0.f ? 0.f : __builtin_amdgcn_exp2f(factors[slot * used + i] - largest);
+            factors[slot * used + i] = factor;
+            total += factor * part; // (a split without a key of finite score sums to zero)
+        }
+        total = wave_sum(total);
+        if (lane == 0)
+            (&totals[0][0])[slot] = total;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < slots * width; i += kWaves * kWave)
+    {
+        const int slot = i / width, c = i % width;
+        const float* column = partial_row(split, unit, 0, slot, width) + 2 + c;
+        const size_t pitch = (size_t) split.row_slots * (width + 2);
+        float numerator = 0.f;
+        constexpr int kAtOnce = 8;
+        for (int w0 = 0; w0 < used; w0 += kAtOnce)
+        {
+            float part[kAtOnce];
+#pragma unroll
+            for (int w = 0; w < kAtOnce; ++w)
+                part[w] = load_shared(column + min(w0 + w, used - 1) * pitch);
+#pragma unroll
+            for (int w = 0; w < kAtOnce; ++w)
+            {
+                const float factor = w0 + w < used ? factors[slot * used + w0 + w] : 0.f;
+                numerator += factor == 0.f ? 0.f : factor * part[w];
+            }
+        }
+        const float denominator = (&totals[0][0])[slot];
+        *out_of(tl, query, head, tl.first + slot, width, c) = denominator == 0.f ? 0.f : numerator / denominator;
+    }
+    if (threadIdx.x == 0) // (zero again for the next launch)
+        __hip_atomic_store(&split.counters[unit], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// The partial rows of a pair's splits joined: a block for each (pair, cached
+// The partial rows of many splits joined by a launch of their own (one block of the
+// last launch would read them too slowly): a block for each (pair, cached
 // head, tile, sequence) of the launch before, whose grid this one's y and z
 // repeat. Its four waves take every fourth split, several in flight.
-constexpr int kJoinWaves = 4;
+constexpr int kJoinWaves = 4, kJoinAhead = 8;
 
-template <int AHEAD>
 __global__ void __launch_bounds__(kJoinWaves* kWave) join_kernel(Cache cache, Rows rows, Query query, Split split,
                                                                  int tile_rows, int first_tile, int first_sequence)
 {
@@ -603,8 +683,8 @@ __global__ void __launch_bounds__(kJoinWaves* kWave) join_kernel(Cache cache, Ro
     if (pair > tl.last || used == 1)
         return;
     const int width = cache.head_width, wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-    const int unit_index = ((int) blockIdx.z * (int) gridDim.y + (int) blockIdx.y) * cache.heads + head;
-    const float* first = partial_row(split, unit_index, 0, slot, width);
+    const int unit = ((int) blockIdx.z * (int) gridDim.y + (int) blockIdx.y) * cache.heads + head;
+    const float* first = partial_row(split, unit, 0, slot, width);
     const size_t pitch = (size_t) split.row_slots * (width + 2);
 
     // Every wave the largest of all; then a wave each fourth split, eight in flight.
@@ -615,11 +695,11 @@ __global__ void __launch_bounds__(kJoinWaves* kWave) join_kernel(Cache cache, Ro
 
     const int c0 = min(lane, width - 1), c1 = min(lane + kWave, width - 1);
     float low = 0.f, high = 0.f, denominator = 0.f;
-    for (int i0 = wave; i0 < used; i0 += AHEAD * kJoinWaves)
+    for (int i0 = wave; i0 < used; i0 += kJoinAhead * kJoinWaves)
     {
-        float top[AHEAD], total[AHEAD], a[AHEAD], b[AHEAD];
+        float top[kJoinAhead], total[kJoinAhead], a[kJoinAhead], b[kJoinAhead];
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i)
+        for (int i = 0; i < kJoinAhead; ++i)
         {
             const float* part = first + min(i0 + i * kJoinWaves, used - 1) * pitch;
             top[i] = part[0];
@@ -628,7 +708,7 @@ __global__ void __launch_bounds__(kJoinWaves* kWave) join_kernel(Cache cache, Ro
             b[i] = part[2 + c1];
         }
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i)
+        for (int i = 0; i < kJoinAhead; ++i)
             if (i0 + i * kJoinWaves < used && total[i] != 0.f) // (a split without a key of finite score sums to zero)
             {
                 const float factor = __builtin_amdgcn_exp2f(top[i] - largest);
@@ -651,9 +731,7 @@ __global__ void __launch_bounds__(kJoinWaves* kWave) join_kernel(Cache cache, Ro
             numerator += sums[w][c];
             total += totals[w];
         }
-        query.out[(size_t) (tl.first_row + pair / query.group) * query.out_stride
-                  + (size_t) (head * query.group + pair % query.group) * width + c] =
-            total == 0.f ? 0.f : numerator / total;
+        *out_of(tl, query, head, pair, width, c) = total == 0.f ? 0.f : numerator / total;
     }
 }
 
@@ -685,15 +763,16 @@ void launch_tiles(hipStream_t stream, dim3 grid, int storage, const Cache& cache
 } // namespace
 
 hipError_t attention(hipStream_t stream, const wsp_paged_cache& cache, const wsp_paged_rows& rows, const float* q,
-                     int q_stride, int heads, bool causal, float scale, float* out, int out_stride, void* scratch,
-                     size_t scratch_bytes)
+                     int q_stride, int heads, bool causal, float scale, float* out, int out_stride,
+                     const Scratch& scratch)
 {
     if (rows.max_count == 0)
         return hipSuccess;
     const Query query {q, q_stride, heads, heads / cache.heads, causal, scale * 1.4426950408889634f, out, out_stride};
     const Plan plan = plan_attention(rows, cache.storage, cache.heads, query.group, cache.head_width,
-                                     scratch_bytes / sizeof(float));
-    const Split split {plan.splits, plan.span, plan.row_slots, static_cast<float*>(scratch)};
+                                     scratch.bytes / sizeof(float));
+    const Split split {plan.splits, plan.span, plan.row_slots, static_cast<float*>(scratch.data),
+                       plan.splits > kFusedSplits ? nullptr : scratch.counters};
     const Cache pool = device_cache(cache);
     const Rows packed = device_rows(rows);
     for (int s = 0; s < rows.sequences; s += plan.slice)
@@ -702,12 +781,11 @@ hipError_t attention(hipStream_t stream, const wsp_paged_cache& cache, const wsp
             const dim3 grid(split.splits * cache.heads, std::min(plan.tiles - t, kMostBlocks),
                             std::min(rows.sequences - s, plan.slice));
             if (plan.tile_rows == kChunkRows)
-                launch_chunks(stream, grid, cache.storage, pool, packed, query, split, t, s);
+                launch_chunks(stream, grid, cache.storage, pool, packed, query, t, s);
             else
                 launch_tiles(stream, grid, cache.storage, pool, packed, query, split, plan.tile_rows, t, s);
-            if (split.splits > 1)
-                (split.splits <= kJoinWaves ? join_kernel<1> : join_kernel<8>)<<<
-                    dim3(cache.heads * split.row_slots, grid.y, grid.z), kJoinWaves * kWave, 0, stream>>>(
+            if (split.splits > kFusedSplits)
+                join_kernel<<<dim3(cache.heads * split.row_slots, grid.y, grid.z), kJoinWaves * kWave, 0, stream>>>(
                     pool, packed, query, split, plan.tile_rows, t, s);
         }
     return hipGetLastError();

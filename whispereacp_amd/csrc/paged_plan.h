@@ -96,6 +96,12 @@ constexpr int kChunkBlocks = 384;
 constexpr int kRoundBlocks = 768; // blocks that run at once, three a CU
 constexpr int kLeastSpan = 256;   // two turns of a block's waves
 constexpr int kMostSpan = 2048;   // lengths differ: blocks of longer spans end apart
+constexpr int kSplitUnits = 4096;  // counters, one for each row tile of a cached head
+constexpr int kJoinRows = 4096;    // partial rows that one block joins
+// Splits that the last block of a row tile joins itself; more are joined by a launch
+// of their own (one token over 131072 positions, 96 splits: 110 us so, 124 by the last
+// block; four tokens over 1500 of 16 streams, three splits: 25 and 23.5).
+constexpr int kFusedSplits = 16;
 constexpr int kMostSequences = 65535; // a launch's z extent
 
 inline Plan plan_attention(const wsp_paged_rows& rows, int storage, int heads, int group, int head_width,
@@ -123,13 +129,14 @@ inline Plan plan_attention(const wsp_paged_rows& rows, int storage, int heads, i
         splits = kRoundBlocks / units;
     if (splits < (rows.max_length + kMostSpan - 1) / kMostSpan)
         splits = (rows.max_length + kMostSpan - 1) / kMostSpan;
+    if (splits > kJoinRows / plan.row_slots)
+        splits = kJoinRows / plan.row_slots;
     if ((unsigned long long) splits > scratch_floats / unit_floats / units)
         splits = (long long) (scratch_floats / unit_floats / units);
-    if (splits < 2)
+    if (splits < 2 || units > kSplitUnits || plan.tile_rows == kChunkRows)
         splits = 1;
-    plan.span = (int) ((rows.max_length + splits - 1) / splits);
-    plan.span = plan.span < kLeastSpan ? kLeastSpan : (plan.span + 63) / 64 * 64;
-    plan.splits = rows.max_length <= plan.span ? 1 : (rows.max_length + plan.span - 1) / plan.span;
+    plan.span = (int) (((rows.max_length + splits - 1) / splits + 31) / 32 * 32);
+    plan.splits = splits == 1 ? 1 : (rows.max_length + plan.span - 1) / plan.span;
     return plan;
 }
 
