@@ -206,13 +206,13 @@ typedef struct wsp_paged_cache
  * pages[s·table_width + p / page_rows]; a page that is not in the pool, or
  * a position past the table, is never touched: append drops the row, read gives
  * NaN, and attention gives NaN for the rows that see such a key. Entries past a
- * sequence's length are not read. */
+ * sequence's length may hold anything. */
 typedef struct wsp_paged_rows
 {
     int sequences;
     int rows;            /* rows the packed tensors hold, at least starts[sequences] */
     int max_count;       /* attention: no sequence has more new rows (more are left as they were) */
-    int max_length;      /* attention: no length is larger (else that sequence's rows are NaN) */
+    int max_length;      /* attention: no length is larger, nor than 2^30 (else that sequence's rows are NaN) */
     int table_width;     /* pages a row of the table names */
     const int* starts;   /* device [sequences + 1] */
     const int* lengths;  /* device [sequences], the new rows among them */

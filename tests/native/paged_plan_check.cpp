@@ -3,6 +3,7 @@
 // arrays. Prints "ok <case>" per passing case; exits 1 on the first failure.
 #include "../../whispereacp_amd/csrc/paged_plan.h"
 
+#include <algorithm>
 #include <climits>
 #include <cstdlib>
 #include <cstring>
@@ -164,5 +165,54 @@ int main()
                && position_of(packed.data(), lengths.data(), 1, 3) == -1,
            "new rows are the last positions");
     expect(shift_of(16) == 4 && shift_of(1024) == 10, "page shifts");
+
+    // Plans: what the launches index fits the scratch, the counters, the join's factors
+    // and a launch's extents, and the splits cover every key a row can see.
+    const size_t scratch = (16 << 20) / sizeof(float);
+    right = true;
+    int split = 0, chunked = 0;
+    for (int storage = WSP_F32; storage <= WSP_E4M3; ++storage)
+        for (int width : {16, 64, 80, 128})
+            for (int heads : {1, 6, 20, 200, 5000})
+                for (int group : {1, 4, 17})
+                    for (int count : {1, 5, 40, 513, 100000, INT_MAX})
+                        for (int sequences : {1, 64, 70000})
+                            for (int length : {0, 1, 255, 257, 448, 9000, 131072, INT_MAX})
+                            {
+                                wsp_paged_cache c = good_cache();
+                                c.storage = storage;
+                                c.head_width = width;
+                                c.heads = heads;
+                                wsp_paged_rows r = good_rows();
+                                r.sequences = sequences;
+                                r.rows = 200000;
+                                r.max_count = count;
+                                r.max_length = length;
+                                r.table_width = 1 << 20;
+                                const Plan p = plan_attention(c, r, group, scratch);
+                                const long long pairs = (long long) std::min(count, r.rows) * group;
+                                const long long units = (long long) p.tiles * heads * p.slice;
+                                right = right && (long long) p.tiles * p.tile_rows >= pairs && p.slice >= 1
+                                        && p.slice <= kMostSequences && p.splits >= 1;
+                                if (p.splits > 1)
+                                {
+                                    ++split;
+                                    right = right
+                                            && (unsigned long long) units * p.splits * p.row_slots * (width + 2) <= scratch
+                                            && units <= kSplitUnits && p.splits * p.row_slots <= kJoinRows
+                                            && p.row_slots >= std::min<long long>(pairs, p.tile_rows)
+                                            && p.span % 32 == 0
+                                            && (long long) p.span * p.splits >= key_bound(r, c.page_rows)
+                                            && p.tile_rows != kChunkRows;
+                                }
+                                chunked += p.tile_rows == kChunkRows;
+                                right = right && (storage != WSP_F32 || p.tile_rows != kChunkRows);
+                            }
+    expect(right && split > 100 && chunked > 100, "plans fit what they index");
+    wsp_paged_rows table_rows = good_rows(); // 2 pages of 16
+    table_rows.max_length = 1000;
+    expect(key_bound(table_rows, 16) == 33, "a row that sees past the table sees one key there");
+    table_rows.max_length = 20;
+    expect(key_bound(table_rows, 16) == 20, "the longest length bounds the keys");
     return 0;
 }

@@ -170,7 +170,7 @@ def test_paged_refusals_and_lookups_on_the_host():
     subprocess.run(["make", "-s", "_build/paged_plan_check"], cwd=os.path.join(ROOT, "tests", "native"), check=True)
     result = subprocess.run([path], capture_output=True, text=True, timeout=60)
     assert result.returncode == 0, result.stdout + result.stderr
-    assert "FAIL" not in result.stdout and result.stdout.count("ok ") >= 33, result.stdout
+    assert "FAIL" not in result.stdout and result.stdout.count("ok ") == 36, result.stdout
 
 
 def test_paged_calls_refuse_without_a_context():

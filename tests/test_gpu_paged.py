@@ -172,25 +172,25 @@ class Case:
         for s, (count, length) in enumerate(zip(self.counts, self.lengths)):
             if count == 0:
                 continue
+            rows = slice(self.starts[s], self.starts[s] + count)
+            positions = np.arange(length - count, length)
+            n = np.where(positions < 0, 0, positions + 1 if causal else length)[:, None]
+            seen = np.arange(max(length, 0))[None, :] < n
             for h in range(self.kv):
                 k, v = self.cached(s, h, 0), self.cached(s, h, 1)
+                largest = np.maximum.accumulate(np.max(np.abs(v), axis=1)) if length > 0 else np.zeros(1)
                 for g in range(self.group):
                     columns = slice((h * self.group + g) * self.width, (h * self.group + g + 1) * self.width)
-                    for i in range(count):
-                        row, position = self.starts[s] + i, length - count + i
-                        n = 0 if position < 0 else position + 1 if causal else length
-                        if n == 0:
-                            out[row, columns] = 0
-                            continue
-                        q = self.q[row, columns].astype(np.float64)
-                        scores = k[:n] @ q * self.scale
-                        p = np.exp(scores - scores.max())
-                        p /= p.sum()
-                        out[row, columns] = p @ v[:n]
-                        a = np.max(np.abs(k[:n]) @ np.abs(q)) * abs(self.scale)
-                        score = a * ((self.width + 8) * 2.0 ** -24 + 2.0 ** -22 + 2.0 ** -23)
-                        bound[row, columns] = (p @ np.abs(v[:n]) * (2 * score + (n + 16) * 2.0 ** -24)
-                                               + n * 2.0 ** -30 * np.max(np.abs(v[:n])))
+                    q = self.q[rows, columns].astype(np.float64)
+                    with np.errstate(invalid="ignore"):
+                        scores = np.where(seen, q @ k.T * self.scale, -np.inf)
+                        p = np.exp(scores - np.where(n > 0, scores.max(axis=1, keepdims=True, initial=-np.inf), 0))
+                        p /= np.where(n > 0, p.sum(axis=1, keepdims=True), 1)
+                    out[rows, columns] = p @ v
+                    a = np.max(np.where(seen, np.abs(q) @ np.abs(k).T, 0), axis=1, initial=0)[:, None] * abs(self.scale)
+                    score = a * ((self.width + 8) * 2.0 ** -24 + 2.0 ** -22 + 2.0 ** -23)
+                    bound[rows, columns] = (p @ np.abs(v) * (2 * score + (n + 16) * 2.0 ** -24)
+                                            + n * 2.0 ** -30 * largest[np.maximum(n - 1, 0)])
         return out, bound
 
 
@@ -394,6 +394,25 @@ def test_attention(ctx, storage, causal, counts, lengths, kv, group, width, page
     check(ctx, Case(storage, counts, lengths, kv, group, width, page, seed=13, spare_rows=spare), causal)
 
 
+# Chunks of many heads, which take the kernel of 128 rows a block (from 384 blocks on).
+CHUNKS = [
+    # counts, lengths, kv, group, width, page, spare rows
+    ([70, 0, 66], [70, 9, 300], 192, 1, 64, 16, 2),
+    ([65, 3], [200, 3], 192, 1, 128, 32, 0),
+    ([40, 129], [90, 130], 64, 3, 96, 64, 1),                       # shared heads, a ragged last tile
+    ([33, 1], [64, 700], 200, 2, 48, 16, 0),                        # narrow heads
+    ([90, 20], [500, 20], 200, 1, 112, 16, 0),
+    ([100, 80], [64, 81], 200, 1, 80, 128, 0),                      # rows before their sequence
+]
+
+
+@pytest.mark.parametrize("storage", STORAGES)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("counts,lengths,kv,group,width,page,spare", CHUNKS)
+def test_attention_of_chunks(ctx, storage, causal, counts, lengths, kv, group, width, page, spare):
+    check(ctx, Case(storage, counts, lengths, kv, group, width, page, seed=83, spare_rows=spare), causal)
+
+
 @pytest.mark.parametrize("storage", STORAGES)
 @pytest.mark.parametrize("count,length", [(1, 5000), (3, 9000), (20, 4100)])
 def test_attention_over_long_sequences(ctx, storage, count, length):
@@ -403,10 +422,11 @@ def test_attention_over_long_sequences(ctx, storage, count, length):
 
 @pytest.mark.parametrize("storage", STORAGES)
 @pytest.mark.parametrize("width", [64, 128])
-def test_attention_of_large_scores(ctx, storage, width):
+@pytest.mark.parametrize("kv", [1, 128])
+def test_attention_of_large_scores(ctx, storage, width, kv):
     # Scores of some hundreds: one key takes nearly all, the running maximum
     # climbs along the keys, and late keys push early ones out.
-    case = Case(storage, [1, 2, 40], [600, 90, 333], 1, 2, width, 32, seed=19)
+    case = Case(storage, [1, 2, 40], [600, 90, 333], kv, 2, width, 32, seed=19)
     case.q *= 40
     for s, n in enumerate(case.lengths):
         for p in range(n):
@@ -417,11 +437,12 @@ def test_attention_of_large_scores(ctx, storage, width):
 
 @pytest.mark.parametrize("storage", ["F16", "BF16", "E4M3", "F32"])
 @pytest.mark.parametrize("q_size,v_size", [(1e-6, 1e4), (1e5, 1e-4), (0.0, 1.0)])
-def test_attention_of_odd_magnitudes(ctx, storage, q_size, v_size):
+@pytest.mark.parametrize("kv", [2, 128])
+def test_attention_of_odd_magnitudes(ctx, storage, q_size, v_size, kv):
     # Queries far from one (their parts are scaled to fp16's range), values large
     # and small. Scores stay ordinary: scale undoes the queries' size.
     # (In fp16 the values stay below its 65504: ten times as many, not 10^4.)
-    case = Case(storage, [1, 33, 5], [70, 100, 5], 2, 1, 64, 16, seed=23)
+    case = Case(storage, [1, 33, 5], [70, 100, 5], kv, 1 if kv == 2 else 2, 64, 16, seed=23)
     v_size = min(v_size, 10.0) if storage == "F16" else v_size
     case.q *= np.float32(q_size)
     case.scale = 0.125 / q_size if q_size else 0.125
@@ -433,8 +454,8 @@ def test_attention_of_odd_magnitudes(ctx, storage, q_size, v_size):
 def test_attention_of_e4m3_rows_of_far_powers(ctx):
     # Rows whose powers of two lie far apart, rows of zeros among them: a
     # weight times its row's power spans more than fp16's range.
-    for count in (1, 40):
-        case = Case("E4M3", [count, 1], [400, 50], 2, 1, 64, 32, seed=29)
+    for count, kv, width in ((1, 2, 64), (40, 2, 64), (70, 192, 64), (70, 192, 96)):
+        case = Case("E4M3", [count, 1], [400, 50], kv, 1, width, 32, seed=29)
         powers = 2.0 ** case.rng.integers(-40, 30, case.value_rows.shape[:3] + (1,))
         case.value_rows *= powers.astype(np.float32)
         case.value_rows[:, :, ::5] *= 0
@@ -445,13 +466,13 @@ def test_attention_of_e4m3_rows_of_far_powers(ctx):
 
 @pytest.mark.parametrize("storage", STORAGES)
 @pytest.mark.parametrize("width", [64, 80, 128])
-@pytest.mark.parametrize("counts,lengths", [([40, 4, 1], [40, 20, 77]), ([200], [300])])
-def test_what_a_row_does_not_see_does_not_reach_it(ctx, storage, width, counts, lengths):
+@pytest.mark.parametrize("counts,lengths,kv", [([40, 4, 1], [40, 20, 77], 2), ([200], [300], 2), ([70, 1], [110, 40], 192)])
+def test_what_a_row_does_not_see_does_not_reach_it(ctx, storage, width, counts, lengths, kv):
     # Infinities and NaN in keys and values: rows before them are as without
     # them, bit for bit; rows that see them are not finite.
-    case = Case(storage, counts, lengths, 2, 1, width, 16, seed=31)
+    case = Case(storage, counts, lengths, kv, 1, width, 16, seed=31)
     clean = check(ctx, case)
-    s = 0
+    s, head = 0, slice(width, 2 * width)
     for row, bad, in_keys in ((counts[0] - 9, np.nan, False), (counts[0] - 14, np.inf, False),
                               (counts[0] - 5, np.nan, True)):
         position = lengths[s] - counts[s] + row
@@ -463,10 +484,11 @@ def test_what_a_row_does_not_see_does_not_reach_it(ctx, storage, width, counts, 
         first = case.starts[s] + row
         assert np.array_equal(got[:first], clean[:first])
         assert np.array_equal(got[:, :width], clean[:, :width])
-        hit = got[first:case.starts[s + 1], width:]
+        assert np.array_equal(got[:, 2 * width:], clean[:, 2 * width:])
+        hit = got[first:case.starts[s + 1], head]
         assert not np.any(np.isfinite(hit if in_keys else hit[:, 5]))
         assert in_keys or np.array_equal(np.delete(hit, 5, 1),
-                                         np.delete(clean[first:case.starts[s + 1], width:], 5, 1)) \
+                                         np.delete(clean[first:case.starts[s + 1], head], 5, 1)) \
             or storage == "E4M3"  # (the row's power is that of its finite values)
         assert np.array_equal(got[case.starts[s + 1]:], clean[case.starts[s + 1]:])
         rows[:] = kept
@@ -487,13 +509,13 @@ def test_keys_of_minus_infinity_weigh_nothing(ctx):
     assert np.allclose(got, want, rtol=1e-4, atol=1e-4)
 
 
-@pytest.mark.parametrize("count", [1, 3, 40])
+@pytest.mark.parametrize("count,kv", [(1, 2), (3, 2), (40, 2), (40, 128)])
 @pytest.mark.parametrize("storage", ["F16", "E4M3"])
-def test_attention_over_bad_pages(ctx, count, storage):
+def test_attention_over_bad_pages(ctx, count, storage, kv):
     # A page outside the pool makes NaN of the rows that see one of its keys, and
     # of no others; so do a table that ends too early and a length past max_length.
     lengths = [150, 150, 150]
-    case = Case(storage, [count] * 3, lengths, 2, 2, 64, 16, seed=41)
+    case = Case(storage, [count] * 3, lengths, kv, 2, 64, 16, seed=41)
     clean = check(ctx, case)
     good = case.table.copy()
     block = (150 - count) // 16  # the new rows' first page
@@ -520,24 +542,30 @@ def test_attention_over_bad_pages(ctx, count, storage):
 
 
 def test_rows_past_max_count_and_past_the_last_sequence_stay(ctx):
-    case = Case("F16", [3, 20], [30, 40], 2, 1, 64, 16, seed=43, spare_rows=4)
-    clean = check(ctx, case)
-    got = attend(ctx, case, rows=case.packed(max_count=4))
-    assert np.array_equal(got[:7], clean[:7]) and np.all(got[7:] == 7.25)
-    got = attend(ctx, case, rows=case.packed(rows=10))
-    assert np.array_equal(got[:10], clean[:10]) and np.all(got[10:] == 7.25)
+    # (A row's last bits may differ where another bound chooses another kernel.)
+    for kv, counts, few in ((2, [3, 20], 4), (192, [3, 90], 70)):
+        case = Case("F16", counts, [30, 100], kv, 1, 64, 16, seed=43, spare_rows=4)
+        want, bound = case.expected(True, check(ctx, case).astype(np.float64))
+        for rows, end in ((case.packed(max_count=few), 3 + few), (case.packed(rows=10), 10)):
+            got = attend(ctx, case, rows=rows)
+            assert np.all(np.abs(got - want)[:end] <= bound[:end]) and np.all(got[end:] == 7.25)
 
 
 @pytest.mark.parametrize("storage", STORAGES)
 def test_strided_tensors_at_odd_floats(ctx, storage):
     import torch
-    case = Case(storage, [1, 35], [200, 40], 2, 2, 64, 16, seed=47)
+    for kv in (2, 192):
+        strided(ctx, Case(storage, [1, 35], [200, 40], kv, 2, 64, 16, seed=47))
+
+
+def strided(ctx, case):
+    import torch
     clean = check(ctx, case)
     n = case.q.shape[1]
     wide = torch.zeros(case.rows * (n + 7) + 1, device="cuda")[1:].view(case.rows, n + 7)
     wide[:, 3:3 + n] = torch.from_numpy(case.q).cuda()
     out = torch.full((case.rows * (n + 5) + 3,), 7.25, device="cuda")[3:].view(case.rows, n + 5)
-    ctx.paged_attention(case.cache(), case.packed(), wide[:, 3:3 + n], 4, True, case.scale, out[:, 1:1 + n])
+    ctx.paged_attention(case.cache(), case.packed(), wide[:, 3:3 + n], 2 * case.kv, True, case.scale, out[:, 1:1 + n])
     torch.cuda.synchronize()
     out = out.cpu().numpy()
     assert np.array_equal(out[:, 1:1 + n], clean)
@@ -612,8 +640,8 @@ def test_a_prompt_and_steps_together(ctx, storage):
 
 
 def test_the_same_bits_every_time(ctx):
-    for count in (1, 7, 64):
-        case = Case("E4M3", [count, count], [2000, 700], 2, 2, 128, 64, seed=71)
+    for count, kv in ((1, 2), (7, 2), (64, 2), (64, 96)):
+        case = Case("E4M3", [count, count], [2000, 700], kv, 2, 128, 64, seed=71)
         cache, rows = case.cache(), case.packed()
         first = attend(ctx, case, cache=cache, rows=rows)
         for _ in range(3):

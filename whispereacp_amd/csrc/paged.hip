@@ -4,6 +4,8 @@
 #include "paged.h"
 #include "paged_device.h"
 
+#include <algorithm>
+
 namespace wsp::paged
 {
 namespace
@@ -115,7 +117,7 @@ struct Place
 __device__ __forceinline__ Place place_of(const Cache& cache, const Rows& rows, int row)
 {
     Place at {-1, -1, 0, false};
-    if (row >= rows.rows)
+    if (row < 0 || row >= rows.rows)
         return at;
     at.sequence = sequence_of(rows.starts, rows.sequences, row);
     if (at.sequence < 0)
@@ -131,11 +133,11 @@ __device__ __forceinline__ Place place_of(const Cache& cache, const Rows& rows, 
 }
 
 template <int ST, int LANES>
-__global__ void __launch_bounds__(kBlock) append_kernel(Cache cache, Rows rows, const float* __restrict__ keys,
+__global__ void __launch_bounds__(kBlock) append_kernel(Cache cache, Rows rows, int first_row, const float* __restrict__ keys,
                                                         int key_stride, const float* __restrict__ values,
                                                         int value_stride)
 {
-    const int row = blockIdx.x * kWavesPerBlock + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int row = first_row + (int) blockIdx.x * kWavesPerBlock + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const Place at = place_of(cache, rows, row);
     if (at.page < 0)
         return;
@@ -189,10 +191,10 @@ __global__ void __launch_bounds__(kBlock) append_kernel(Cache cache, Rows rows, 
 }
 
 template <int ST, int LANES>
-__global__ void __launch_bounds__(kBlock) read_kernel(Cache cache, Rows rows, float* __restrict__ keys,
+__global__ void __launch_bounds__(kBlock) read_kernel(Cache cache, Rows rows, int first_row, float* __restrict__ keys,
                                                       int key_stride, float* __restrict__ values, int value_stride)
 {
-    const int row = blockIdx.x * kWavesPerBlock + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int row = first_row + (int) blockIdx.x * kWavesPerBlock + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const Place at = place_of(cache, rows, row);
     if (at.sequence < 0)
         return;
@@ -242,17 +244,23 @@ __global__ void __launch_bounds__(kBlock) read_kernel(Cache cache, Rows rows, fl
     }
 }
 
-// f called with the storage and the lanes of a head as compile-time constants, and
-// the grid: rows, and the heads that a wave does not take.
+// f called with the storage and the lanes of a head as compile-time constants, the
+// grid (rows, and the heads that a wave does not take) and the first row, as often as
+// a launch's x extent takes.
+constexpr int kMostRows = 1 << 24;
+
 template <class F>
 void by_lanes(const wsp_paged_cache& cache, const wsp_paged_rows& rows, F&& f)
 {
     by_storage(cache.storage, [&](auto storage) {
         auto run = [&](auto lanes) {
             constexpr int kHeads = kTurns * kWave / decltype(lanes)::value;
-            f(storage, lanes,
-              dim3((unsigned) (((long long) rows.rows + kWavesPerBlock - 1) / kWavesPerBlock),
-                   (cache.heads + kHeads - 1) / kHeads));
+            for (long long first = 0; first < rows.rows; first += kMostRows)
+            {
+                const int count = (int) std::min<long long>(rows.rows - first, kMostRows);
+                f(storage, lanes,
+                  dim3((count + kWavesPerBlock - 1) / kWavesPerBlock, (cache.heads + kHeads - 1) / kHeads), (int) first);
+            }
         };
         cache.head_width <= 64 ? run(std::integral_constant<int, 16> {}) : run(std::integral_constant<int, 32> {});
     });
@@ -262,9 +270,9 @@ void by_lanes(const wsp_paged_cache& cache, const wsp_paged_rows& rows, F&& f)
 hipError_t append(hipStream_t stream, const wsp_paged_cache& cache, const wsp_paged_rows& rows, const float* keys,
                   int key_stride, const float* values, int value_stride)
 {
-    by_lanes(cache, rows, [&](auto storage, auto lanes, dim3 grid) {
+    by_lanes(cache, rows, [&](auto storage, auto lanes, dim3 grid, int first) {
         append_kernel<storage(), lanes()><<<grid, kBlock, 0, stream>>>(
-            device_cache(cache), device_rows(rows), keys, key_stride, values, value_stride);
+            device_cache(cache), device_rows(cache, rows), first, keys, key_stride, values, value_stride);
     });
     return hipGetLastError();
 }
@@ -272,9 +280,9 @@ hipError_t append(hipStream_t stream, const wsp_paged_cache& cache, const wsp_pa
 hipError_t read(hipStream_t stream, const wsp_paged_cache& cache, const wsp_paged_rows& rows, float* keys,
                 int key_stride, float* values, int value_stride)
 {
-    by_lanes(cache, rows, [&](auto storage, auto lanes, dim3 grid) {
+    by_lanes(cache, rows, [&](auto storage, auto lanes, dim3 grid, int first) {
         read_kernel<storage(), lanes()><<<grid, kBlock, 0, stream>>>(
-            device_cache(cache), device_rows(rows), keys, key_stride, values, value_stride);
+            device_cache(cache), device_rows(cache, rows), first, keys, key_stride, values, value_stride);
     });
     return hipGetLastError();
 }

@@ -36,6 +36,7 @@ struct RowTile
     int pairs;       // rows to compute times group
     int past;        // position of the first new row (before 0: none)
     int length;
+    int bound;       // no row looks further (Rows::key_bound)
     int first, last; // this tile's pairs
     int least, most; // keys that its first and its last row see
     bool poisoned;   // the length passes max_length
@@ -44,19 +45,21 @@ struct RowTile
 __device__ __forceinline__ int keys_seen(const Query& query, const RowTile& t, int pair)
 {
     const long long position = (long long) t.past + pair / query.group;
-    return position < 0 ? 0 : query.causal ? (int) position + 1 : t.length;
+    return position < 0 ? 0 : min(query.causal ? (int) position + 1 : t.length, t.bound);
 }
 
 // False where the tile has no row.
 __device__ __forceinline__ bool find_tile(const Rows& rows, const Query& query, int sequence, int tile, int tile_rows,
                                           RowTile& t)
 {
+    // (All three in flight at once.)
     t.first_row = rows.starts[sequence];
     const int end = rows.starts[sequence + 1];
+    t.length = rows.lengths[sequence];
+    t.bound = rows.key_bound;
     if (t.first_row < 0 || end <= t.first_row)
         return false;
     const int count = end - t.first_row;
-    t.length = rows.lengths[sequence];
     t.past = max(t.length, 0) - count;
     t.pairs = min(min(count, rows.max_count), rows.rows - t.first_row) * query.group;
     t.first = tile * tile_rows;

@@ -66,21 +66,15 @@ struct Tile // one lane's part of 32 keys and values, as stored
     bool bad[2];                                 // the page of keys 16b .. is none
 };
 
-// The pages of keys k0 .. k0 + 15 and k0 + 16 .. k0 + 31 (-1: none). k0 is below
-// `end`; of a sixteen that begins at or past it the first is named again (nothing
-// there counts).
+// The pages of keys k0 .. k0 + 15 and k0 + 16 .. k0 + 31 (-1: none).
 struct Pages
 {
     int page[2];
 };
-__device__ __forceinline__ int second_key(int k0, int end)
-{
-    return k0 + 16 < end ? k0 + 16 : k0;
-}
-__device__ __forceinline__ Pages find_pages(const Cache& cache, const int* table, int table_width, int k0, int end)
+__device__ __forceinline__ Pages find_pages(const Cache& cache, const int* table, int table_width, int k0)
 {
     return {{page_of(table, table_width, cache.page_shift, cache.pages, k0),
-             page_of(table, table_width, cache.page_shift, cache.pages, second_key(k0, end))}};
+             page_of(table, table_width, cache.page_shift, cache.pages, k0 + 16)}};
 }
 
 // Where a lane's parts of a key and of a value row lie in a sixteen's rows, in bytes.
@@ -89,8 +83,9 @@ struct Offsets
     uint32_t key, value;
 };
 
-// Keys and values k0 .. k0 + 31 of a cached head. (The pages are the same for the
-// wave: what is not in `at` is scalar.)
+// Keys and values k0 .. k0 + 31 of a cached head. k0 is below `end`; of a sixteen
+// that begins at or past it the first is read again (nothing there counts). (The pages
+// are the same for the wave: what is not in `at` is scalar.)
 template <int ST, int W, bool FULL>
 __device__ __forceinline__ void load_tile(const Cache& cache, const Pages& pages, int head, int k0, int end, Offsets at,
                                           Tile<ST, W>& t)
@@ -100,9 +95,10 @@ __device__ __forceinline__ void load_tile(const Cache& cache, const Pages& pages
 #pragma unroll
     for (int b = 0; b < 2; ++b)
     {
-        t.bad[b] = pages.page[b] < 0;
-        const size_t row = pool_row(max(pages.page[b], 0), head, (b == 0 ? k0 : second_key(k0, end)) & mask, cache.heads,
-                                    cache.page_shift);
+        const bool second = b == 1 && k0 + 16 < end;
+        const int page = second ? pages.page[1] : pages.page[0];
+        t.bad[b] = page < 0;
+        const size_t row = pool_row(max(page, 0), head, (second ? k0 + 16 : k0) & mask, cache.heads, cache.page_shift);
         const char* keys = static_cast<const char*>(cache.keys) + row * row_bytes;
         const char* values = static_cast<const char*>(cache.values) + row * row_bytes;
         constexpr int kRuns = W * bytes_of<ST> / 64;
@@ -181,17 +177,34 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
     const int unit = ((int) blockIdx.z * (int) gridDim.y + (int) blockIdx.y) * cache.heads + head;
     const int sequence = first_sequence + blockIdx.z;
     const int tile = first_tile + (int) (gridDim.y - 1 - blockIdx.y); // (the tiles that see most come first)
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int lane = threadIdx.x % kWave, li = lane % 16, g = lane / 16;
+    const int width = FULL ? W : cache.head_width;
+    // A block's start is a chain of round trips to memory: the first keys' pages are
+    // looked up beside the sequence's starts and length, and the first keys and values
+    // are in flight while the queries arrive and are cut.
+    const int* table = rows.pages + (size_t) sequence * rows.table_width;
+    constexpr int kStride = kKeys * kWaves;
+    const int begin = which * split.span;
+    int k0 = begin + kKeys * wave;
+    Pages pages = find_pages(cache, table, rows.table_width, k0);
     RowTile tl;
     if (!find_tile(rows, query, sequence, tile, 16 * QT, tl))
         return;
     const int used = splits_used(tl, split.span);
     if (which >= used)
         return;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int lane = threadIdx.x % kWave, li = lane % 16, g = lane / 16;
-    const int width = FULL ? W : cache.head_width;
-    const int* table = rows.pages + (size_t) sequence * rows.table_width;
-    const int begin = which * split.span, end = tl.poisoned ? 0 : min(begin + split.span, tl.most);
+    const int end = tl.poisoned ? 0 : min(begin + split.span, tl.most);
+    // (Value lanes past the row read its start: they hold channels nobody stores.)
+    const int row_bytes = width * bytes_of<ST>, channel = FULL || li * CPL < width ? li * CPL : 0;
+    const Offsets at {(uint32_t) (li * row_bytes + 16 * g), (uint32_t) (4 * g * row_bytes + channel * bytes_of<ST>)};
+    Tile<ST, W> now;
+    if (k0 < end)
+    {
+        load_tile<ST, W, FULL>(cache, pages, head, k0, end, at, now);
+        if (k0 + kStride < end)
+            pages = find_pages(cache, table, rows.table_width, k0 + kStride);
+    }
 
     // The queries: lane (li, g) holds the channels of pair li that it holds of a key.
     uint32_t qp[QT][OT == kF32 ? 1 : kParts][OT == kF32 ? W / 4 : W / 8];
@@ -204,16 +217,16 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
         const bool real = pair <= tl.last;
         seen[t] = real ? min(keys_seen(query, tl, pair), end) : end;
         float x[W / 4];
-        const float* at = query.q + (size_t) (tl.first_row + (real ? pair : tl.first) / query.group) * query.q_stride
+        const float* from = query.q + (size_t) (tl.first_row + (real ? pair : tl.first) / query.group) * query.q_stride
                           + (size_t) (head * query.group + (real ? pair : tl.first) % query.group) * width;
 #pragma unroll
         for (int i = 0; i < W / 4; i += 4)
         {
             constexpr int kRun = 16 / bytes_of<ST>;
-            const int channel = (4 * (i / kRun) + g) * kRun + i % kRun;
+            const int c = (4 * (i / kRun) + g) * kRun + i % kRun;
             float4v run = {0.f, 0.f, 0.f, 0.f};
-            if (real && (FULL || channel < width))
-                run = *reinterpret_cast<const float4u*>(at + channel);
+            if (real && (FULL || c < width))
+                run = *reinterpret_cast<const float4u*>(from + c);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 x[i + j] = run[j] * query.scale;
@@ -505,19 +518,9 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
 
     // The next keys are in flight while these are worked on (not where two tiles
     // do not fit the registers), and the pages of those behind them looked up.
-    constexpr int kStride = kKeys * kWaves;
     constexpr bool kAhead = ST != kF32 || W == 64;
-    int k0 = begin + kKeys * wave;
     if (k0 < end)
     {
-        // (Value lanes past the row read its start: they hold channels nobody stores.)
-        const int row_bytes = width * bytes_of<ST>, channel = FULL || li * CPL < width ? li * CPL : 0;
-        const Offsets at {(uint32_t) (li * row_bytes + 16 * g), (uint32_t) (4 * g * row_bytes + channel * bytes_of<ST>)};
-        Tile<ST, W> now;
-        Pages pages = find_pages(cache, table, rows.table_width, k0, end);
-        load_tile<ST, W, FULL>(cache, pages, head, k0, end, at, now);
-        if (k0 + kStride < end)
-            pages = find_pages(cache, table, rows.table_width, k0 + kStride, end);
         for (; k0 + kStride < end; k0 += kStride)
         {
             if constexpr (!kAhead)
@@ -525,7 +528,7 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
             Tile<ST, W> next;
             load_tile<ST, W, FULL>(cache, pages, head, k0 + kStride, end, at, next);
             if (k0 + 2 * kStride < end)
-                pages = find_pages(cache, table, rows.table_width, k0 + 2 * kStride, end);
+                pages = find_pages(cache, table, rows.table_width, k0 + 2 * kStride);
             if constexpr (kAhead)
             {
                 __builtin_amdgcn_sched_barrier(0);
@@ -769,12 +772,11 @@ hipError_t attention(hipStream_t stream, const wsp_paged_cache& cache, const wsp
     if (rows.max_count == 0)
         return hipSuccess;
     const Query query {q, q_stride, heads, heads / cache.heads, causal, scale * 1.4426950408889634f, out, out_stride};
-    const Plan plan = plan_attention(rows, cache.storage, cache.heads, query.group, cache.head_width,
-                                     scratch.bytes / sizeof(float));
+    const Plan plan = plan_attention(cache, rows, query.group, scratch.bytes / sizeof(float));
     const Split split {plan.splits, plan.span, plan.row_slots, static_cast<float*>(scratch.data),
                        plan.splits > kFusedSplits ? nullptr : scratch.counters};
     const Cache pool = device_cache(cache);
-    const Rows packed = device_rows(rows);
+    const Rows packed = device_rows(cache, rows);
     for (int s = 0; s < rows.sequences; s += plan.slice)
         for (int t = 0; t < plan.tiles; t += kMostBlocks)
         {

@@ -91,8 +91,14 @@ __device__ __forceinline__ u32x4 e4m3_run(uint32_t low, uint32_t high, float pow
                   pair(high, std::true_type {})};
 }
 
-template <int ST, int W, bool FULL>
-__global__ void __launch_bounds__(kChunkWaves* kWave, 2)
+// Waves a SIMD: two, or one where the registers of two would spill into the loop.
+template <int ST, int C, bool FULL>
+constexpr int kChunkOccupancy = (ST == kBF16 && C >= 96) || (!FULL && C == 128) ? 1 : 2;
+
+// Heads lie in LDS as W channels (64 or 128), of which C are worked on (a multiple of
+// 32); FULL: the heads are C wide.
+template <int ST, int W, int C, bool FULL>
+__global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FULL>))
     chunk_attention_kernel(Cache cache, Rows rows, Query query, int first_tile, int first_sequence)
 {
     constexpr int OT = operand_of<ST>, kParts = parts_of<OT>();
@@ -117,7 +123,7 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, 2)
         return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int lane = threadIdx.x % kWave, n = lane % 32, h = lane / 32;
-    const int width = FULL ? W : cache.head_width, row_bytes = width * bytes_of<ST>;
+    const int width = FULL ? C : cache.head_width, row_bytes = width * bytes_of<ST>;
     const int page_mask = (1 << cache.page_shift) - 1;
     const int* table = rows.pages + (size_t) sequence * rows.table_width;
     const int end = tl.poisoned ? 0 : tl.most;
@@ -130,15 +136,15 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, 2)
     const int seen = real ? min(keys_seen(query, tl, pair), end) : 0;
     const int wave_least = first <= tl.last ? min(keys_seen(query, tl, first), end) : 0;
     const int wave_most = first <= tl.last ? min(keys_seen(query, tl, min(first + 31, tl.last)), end) : 0;
-    u32x4 qp[W / 16][kParts];
+    u32x4 qp[C / 16][kParts];
     float unit = 1.f; // the power of two that the parts leave out
     {
         const float* at = query.q + (size_t) (tl.first_row + (real ? pair : tl.first) / query.group) * query.q_stride
                           + (size_t) (head * query.group + (real ? pair : tl.first) % query.group) * width;
-        float x[W / 16][8];
+        float x[C / 16][8];
         float top = 0.f;
 #pragma unroll
-        for (int j = 0; j < W / 16; ++j)
+        for (int j = 0; j < C / 16; ++j)
 #pragma unroll
             for (int i = 0; i < 8; i += 4)
             {
@@ -161,7 +167,7 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, 2)
             unit = ldexpf(1.f, -shift);
         }
 #pragma unroll
-        for (int j = 0; j < W / 16; ++j)
+        for (int j = 0; j < C / 16; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
             {
@@ -182,9 +188,12 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, 2)
     constexpr int kKeysAtOnce = kThreads / (W / 8); // 16 or 32
     const int key_run = threadIdx.x % (W / 8), key_of = threadIdx.x / (W / 8);
     const int value_channel = threadIdx.x % 32 * kValueChannels, value_run = 2 * wave + h;
-    const bool key_real = FULL || 8 * key_run < width;
-    const uint32_t key_offset = key_of % 16 * row_bytes + 8 * key_run * bytes_of<ST>;
-    const uint32_t value_offset = 4 * h * row_bytes + (FULL || value_channel < width ? value_channel : 0) * bytes_of<ST>;
+    // (Lanes past the row read its start: keys' runs there are staged as zeros, values'
+    // channels there reach no output.)
+    const bool key_real = (FULL && C == W) || 8 * key_run < width;
+    const uint32_t key_offset = key_of % 16 * row_bytes + (key_real ? 8 * key_run : 0) * bytes_of<ST>;
+    const uint32_t value_offset =
+        4 * h * row_bytes + ((FULL && C == W) || value_channel < width ? value_channel : 0) * bytes_of<ST>;
     struct Raw
     {
         uint32_t k[kKeyRuns][kKeyWords];
@@ -211,12 +220,7 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, 2)
             const int page = kKeysAtOnce == 16 ? pages[i] : i == 0 ? (second ? pages[1] : pages[0])
                                                                    : (second ? pages[3] : pages[2]);
             const size_t row = row_of(page, k0 + kKeysAtOnce * i + (second ? 16 : 0));
-            if (key_real)
-                load_words(static_cast<const char*>(cache.keys) + row * row_bytes + key_offset, raw.k[i]);
-            else
-#pragma unroll
-                for (int j = 0; j < kKeyWords; ++j)
-                    raw.k[i][j] = 0;
+            load_words(static_cast<const char*>(cache.keys) + row * row_bytes + key_offset, raw.k[i]);
             if constexpr (ST == kE4M3)
                 raw.ke[i] = *global(cache.key_exponents + row + (uint32_t) (key_of % 16));
         }
@@ -336,6 +340,8 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, 2)
                                apart ? 1.f : __uint_as_float(power_bits(raw.ke[i], key_base)));
             else
                 run = u32x4 {raw.k[i][0], raw.k[i][1], raw.k[i][2], raw.k[i][3]};
+            if (!key_real)
+                run = u32x4 {0, 0, 0, 0};
             ks[key_slot<W>(key_of + kKeysAtOnce * i, key_run)] = run;
         }
         // Values as pairs of channels, then pairs of keys of one channel.
@@ -390,9 +396,9 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, 2)
         }
     };
 
-    float16v o[W / 32];
+    float16v o[C / 32];
 #pragma unroll
-    for (int c = 0; c < W / 32; ++c)
+    for (int c = 0; c < C / 32; ++c)
         o[c] = float16v {};
     float m = -INFINITY, l = 0.f;
     if (threadIdx.x == 0)
@@ -425,12 +431,12 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, 2)
                 break;
             __builtin_amdgcn_s_setprio(1);
             float16v s = {};
-            u32x4 key[W / 16];
+            u32x4 key[C / 16];
 #pragma unroll
-            for (int j = 0; j < W / 16; ++j)
+            for (int j = 0; j < C / 16; ++j)
                 key[j] = ks[key_slot<W>(32 * b + n, 2 * j + h)];
 #pragma unroll
-            for (int j = 0; j < W / 16; ++j)
+            for (int j = 0; j < C / 16; ++j)
 #pragma unroll
                 for (int p = kParts - 1; p >= 0; --p)
                     s = mfma32<OT>(key[j], qp[j][p], s);
@@ -474,7 +480,7 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, 2)
                 const float alpha = __builtin_amdgcn_exp2f(m - finite);
                 l *= alpha;
 #pragma unroll
-                for (int c = 0; c < W / 32; ++c)
+                for (int c = 0; c < C / 32; ++c)
                     o[c] *= alpha;
                 m = m_new;
             }
@@ -514,14 +520,14 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, 2)
 #pragma unroll
             for (int t = 0; t < 2; ++t)
             {
-                u32x4 value[W / 32];
+                u32x4 value[C / 32];
 #pragma unroll
-                for (int c = 0; c < W / 32; ++c)
+                for (int c = 0; c < C / 32; ++c)
                     value[c] = vs[value_slot(32 * c + n, 4 * b + 2 * t + h)];
 #pragma unroll
                 for (int p = kParts - 1; p >= 0; --p)
 #pragma unroll
-                    for (int c = 0; c < W / 32; ++c)
+                    for (int c = 0; c < C / 32; ++c)
                         o[c] = mfma32<OT>(value[c], weights[t][p], o[c]);
             }
             __builtin_amdgcn_s_setprio(0);
@@ -551,7 +557,7 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, 2)
                         continue;
                     const size_t row = pool_row(page, head, position & page_mask, cache.heads, cache.page_shift);
 #pragma unroll
-                    for (int c = 0; c < W / 32; ++c)
+                    for (int c = 0; c < C / 32; ++c)
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
                         {
@@ -576,7 +582,7 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, 2)
     const float by = l == 0.f ? 0.f : power / l;
     float* const out = out_of(tl, query, head, pair, width, 0);
 #pragma unroll
-    for (int c = 0; c < W / 32; ++c)
+    for (int c = 0; c < C / 32; ++c)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (FULL || 32 * c + 8 * i + 4 * h < width)
@@ -589,17 +595,19 @@ void launch_chunks(hipStream_t stream, dim3 grid, int storage, const Cache& cach
                    const Query& query, int first_tile, int first_sequence)
 {
     by_storage(storage, [&](auto type) {
-        auto run = [&](auto width, auto full) {
+        auto run = [&](auto width, auto channels, auto full) {
             if constexpr (type() != kF32)
-                chunk_attention_kernel<type(), width(), full()><<<grid, kChunkWaves * kWave, 0, stream>>>(
+                chunk_attention_kernel<type(), width(), channels(), full()><<<grid, kChunkWaves * kWave, 0, stream>>>(
                     cache, rows, query, first_tile, first_sequence);
         };
         using Narrow = std::integral_constant<int, 64>;
+        using Middle = std::integral_constant<int, 96>;
         using Wide = std::integral_constant<int, 128>;
-        cache.head_width == 64    ? run(Narrow {}, std::true_type {})
-        : cache.head_width == 128 ? run(Wide {}, std::true_type {})
-        : cache.head_width < 64   ? run(Narrow {}, std::false_type {})
-                                  : run(Wide {}, std::false_type {});
+        cache.head_width == 64    ? run(Narrow {}, Narrow {}, std::true_type {})
+        : cache.head_width == 128 ? run(Wide {}, Wide {}, std::true_type {})
+        : cache.head_width < 64   ? run(Narrow {}, Narrow {}, std::false_type {})
+        : cache.head_width <= 96  ? run(Wide {}, Middle {}, std::false_type {})
+                                  : run(Wide {}, Wide {}, std::false_type {});
     });
 }
 } // namespace wsp::paged

@@ -23,7 +23,7 @@ struct Cache
 };
 struct Rows
 {
-    int sequences, rows, max_count, max_length, table_width;
+    int sequences, rows, max_count, max_length, key_bound, table_width;
     const int* starts;
     const int* lengths;
     const int* pages;
@@ -40,9 +40,10 @@ inline Cache device_cache(const wsp_paged_cache& c)
     return {c.pages, shift_of(c.page_rows), c.heads, c.head_width, c.keys, c.values, c.key_exponents, c.value_exponents};
 }
 
-inline Rows device_rows(const wsp_paged_rows& r)
+inline Rows device_rows(const wsp_paged_cache& c, const wsp_paged_rows& r)
 {
-    return {r.sequences, r.rows, r.max_count, r.max_length, r.table_width, r.starts, r.lengths, r.pages};
+    return {r.sequences,   r.rows,   r.max_count, r.max_length < kMostLength ? r.max_length : kMostLength,
+            key_bound(r, c.page_rows), r.table_width, r.starts,    r.lengths, r.pages};
 }
 
 // f called with the storage as a compile-time constant.

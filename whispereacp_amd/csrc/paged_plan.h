@@ -80,6 +80,18 @@ inline int say(char* why, size_t size, int code, const char* format, ...)
     return code;
 }
 
+// Positions past this are not attended (a length past it counts as past max_length).
+constexpr int kMostLength = 1 << 30;
+
+// Keys that an attention call can meet: max_length, and of a table that ends before it
+// one key past the table, which makes NaN of the rows that see it.
+inline int key_bound(const wsp_paged_rows& rows, int page_rows)
+{
+    const long long held = (long long) rows.table_width * page_rows + 1;
+    long long bound = rows.max_length < kMostLength ? rows.max_length : kMostLength;
+    return (int) (bound < held ? bound : held);
+}
+
 // How an attention call is cut: blocks of tile_rows pairs (new row, query head
 // of a cached head's group), `splits` blocks of `span` keys along the keys, and
 // launches of at most `slice` sequences. Splits leave partial rows of
@@ -95,7 +107,7 @@ constexpr int kChunkRows = 128;   // of the kernel for many rows
 constexpr int kChunkBlocks = 384;
 constexpr int kRoundBlocks = 768; // blocks that run at once, three a CU
 constexpr int kLeastSpan = 256;   // two turns of a block's waves
-constexpr int kMostSpan = 2048;   // lengths differ: blocks of longer spans end apart
+constexpr int kMostSpan = 4096;   // lengths differ: blocks of longer spans end apart
 constexpr int kSplitUnits = 4096;  // counters, one for each row tile of a cached head
 constexpr int kJoinRows = 4096;    // partial rows that one block joins
 // Splits that the last block of a row tile joins itself; more are joined by a launch
@@ -104,11 +116,12 @@ constexpr int kJoinRows = 4096;    // partial rows that one block joins
 constexpr int kFusedSplits = 16;
 constexpr int kMostSequences = 65535; // a launch's z extent
 
-inline Plan plan_attention(const wsp_paged_rows& rows, int storage, int heads, int group, int head_width,
-                           size_t scratch_floats)
+inline Plan plan_attention(const wsp_paged_cache& cache, const wsp_paged_rows& rows, int group, size_t scratch_floats)
 {
     Plan plan {};
-    const long long pairs = (long long) rows.max_count * group;
+    const int storage = cache.storage, heads = cache.heads, head_width = cache.head_width;
+    const long long pairs = (long long) (rows.max_count < rows.rows ? rows.max_count : rows.rows) * group;
+    const int keys = key_bound(rows, cache.page_rows);
     // Blocks of 128 rows where they make a round and a half of the chip: each takes
     // longer (16 sequences of 512 rows over 2048 keys of 12 heads of 64, fp16: 128 us and 176
     // in blocks of 32; 4 sequences 87 and 55; 64 of 32 rows over 4096, heads of 128 in
@@ -124,19 +137,19 @@ inline Plan plan_attention(const wsp_paged_rows& rows, int storage, int heads, i
     const long long units = (long long) plan.tiles * heads * plan.slice;
     const size_t unit_floats = (size_t) plan.row_slots * (head_width + 2);
     // As many splits as still run at once, or as keep the spans short.
-    long long splits = (rows.max_length + kLeastSpan - 1) / kLeastSpan;
+    long long splits = (keys + kLeastSpan - 1) / kLeastSpan;
     if (splits > kRoundBlocks / units)
         splits = kRoundBlocks / units;
-    if (splits < (rows.max_length + kMostSpan - 1) / kMostSpan)
-        splits = (rows.max_length + kMostSpan - 1) / kMostSpan;
+    if (splits < (keys + kMostSpan - 1) / kMostSpan)
+        splits = (keys + kMostSpan - 1) / kMostSpan;
     if (splits > kJoinRows / plan.row_slots)
         splits = kJoinRows / plan.row_slots;
     if ((unsigned long long) splits > scratch_floats / unit_floats / units)
         splits = (long long) (scratch_floats / unit_floats / units);
     if (splits < 2 || units > kSplitUnits || plan.tile_rows == kChunkRows)
         splits = 1;
-    plan.span = (int) (((rows.max_length + splits - 1) / splits + 31) / 32 * 32);
-    plan.splits = splits == 1 ? 1 : (rows.max_length + plan.span - 1) / plan.span;
+    plan.span = (int) (((keys + splits - 1) / splits + 31) / 32 * 32);
+    plan.splits = splits == 1 ? 1 : (keys + plan.span - 1) / plan.span;
     return plan;
 }
 
