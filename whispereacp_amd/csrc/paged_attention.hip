@@ -391,15 +391,24 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
                 }
         }
 
-        // The rows, two channels of each lane's at a time.
+        // The rows, two channels of each lane's at a time. A weight of zero hides a value
+        // only while it is finite: the careful way counts values that no pair sees as
+        // zero, and where some pairs see a key and others do not, non-finite values are
+        // added behind the products, to those that see them alone.
         bool odd = false;
+        const bool mixed = careful && tl.least < tl.most;
+        uint32_t shown[4]; // of keys 2d and 2d + 1 of a lane's eight: all bits of those that some pair sees
+        if (careful)
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+            {
+                const int key = k0 + 16 * (d / 2) + 4 * g + 2 * (d % 2);
+                shown[d] = kv.bad[d / 2] ? 0u : (key < end ? 0xFFFFu : 0u) | (key + 1 < end ? 0xFFFF0000u : 0u);
+            }
 #pragma unroll
         for (int c = 0; c < CPL; c += 2)
         {
-            // Channels CPL·li + c and + c + 1 of keys 16b + 4g + r. A weight of zero
-            // hides a value only while it is finite: the careful way counts values
-            // that no pair sees as zero, and non-finite ones that some pair sees are
-            // added behind the products, to those pairs alone.
+            // Channels CPL·li + c and + c + 1 of keys 16b + 4g + r.
             if constexpr (OT == kF32)
             {
                 float v[2][8];
@@ -411,15 +420,19 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
                 if (careful)
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                    {
-                        const bool unseen = k0 + 16 * (i / 4) + 4 * g + i % 4 >= end || kv.bad[i / 4];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if ((shown[i / 2] & (i % 2 == 0 ? 0xFFFFu : 0xFFFF0000u)) == 0)
+                                v[e][i] = 0.f;
+                if (mixed)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
 #pragma unroll
                         for (int e = 0; e < 2; ++e)
                         {
-                            odd = odd || (!unseen && !isfinite(v[e][i]));
-                            v[e][i] = unseen || !isfinite(v[e][i]) ? 0.f : v[e][i];
+                            odd = odd || !isfinite(v[e][i]);
+                            v[e][i] = isfinite(v[e][i]) ? v[e][i] : 0.f;
                         }
-                    }
 #pragma unroll
                 for (int t = 0; t < QT; ++t)
 #pragma unroll
@@ -444,18 +457,20 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
                 }
                 if (careful)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                    {
-                        const bool unseen = k0 + 16 * (i / 4) + 4 * g + i % 4 >= end || kv.bad[i / 4];
-                        const uint32_t half = i % 2 == 0 ? 0xFFFFu : 0xFFFF0000u;
+                    for (int d = 0; d < 4; ++d)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            v[e][d] &= shown[d];
+                if (mixed)
+#pragma unroll
+                    for (int d = 0; d < 4; ++d)
 #pragma unroll
                         for (int e = 0; e < 2; ++e)
                         {
-                            const uint32_t kept = unseen ? 0u : finite_halves<OT>(v[e][i / 2] & half);
-                            odd = odd || (!unseen && kept != (v[e][i / 2] & half));
-                            v[e][i / 2] = (v[e][i / 2] & ~half) | kept;
+                            const uint32_t kept = finite_halves<OT>(v[e][d]);
+                            odd = odd || kept != v[e][d];
+                            v[e][d] = kept;
                         }
-                    }
 #pragma unroll
                 for (int t = 0; t < QT; ++t)
 #pragma unroll
@@ -470,7 +485,7 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
                     }
             }
         }
-        if (careful && __any(odd)) // (rare: infinities or NaN among the new rows' values)
+        if (mixed && __any(odd)) // (rare: infinities or NaN among the new rows' values)
 #pragma unroll
             for (int t = 0; t < QT; ++t)
             {
