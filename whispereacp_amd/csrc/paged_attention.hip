@@ -295,7 +295,8 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
                     float4v part[4];
 #pragma unroll
                     for (int i = 0; i < W / 4; ++i)
-                        part[i % 4] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                        if (FULL || i < 4 || 16 * (i / 4) < width) // (past the row there are zeros)
+                            part[i % 4] = __builtin_amdgcn_mfma_f32_16x16x4f32(
                             __uint_as_float(kv.k[b][i]), __uint_as_float(qp[t][0][i]),
                             i < 4 ? float4v {0.f, 0.f, 0.f, 0.f} : part[i % 4], 0, 0, 0);
                     s[b] = (part[0] + part[1]) + (part[2] + part[3]);
