@@ -193,7 +193,8 @@ int main()
                                 const long long pairs = (long long) std::min(count, r.rows) * group;
                                 const long long units = (long long) p.tiles * heads * p.slice;
                                 right = right && (long long) p.tiles * p.tile_rows >= pairs && p.slice >= 1
-                                        && p.slice <= kMostSequences && p.splits >= 1;
+                                        && p.slice <= kMostSequences && p.splits >= 1 && p.span >= 32
+                                        && (p.splits > 1 || p.span >= key_bound(r, c.page_rows));
                                 if (p.splits > 1)
                                 {
                                     ++split;

@@ -464,6 +464,39 @@ def test_attention_of_e4m3_rows_of_far_powers(ctx):
         check(ctx, case)
 
 
+@pytest.mark.parametrize("kv", [2, 192])
+@pytest.mark.parametrize("first,others", [(0, -15), (0, -22), (-80, -7), (-80, 100), (100, -30)])
+def test_attention_of_e4m3_rows_far_from_the_first(ctx, kv, first, others):
+    # The first key's and value's rows have power `first`, about, and the key nearly no
+    # weight; all others' lie near `others`, among them fp16's least numbers as operands
+    # and rows past its range. They keep an accuracy of their own: the bound is the one
+    # above with A = 0.125·(4·60 + 63·16), the largest of |q| and |k| being four in
+    # units of the others, and the others' values alone.
+    case = Case("E4M3", [70, 1], [200, 90], kv, 1, 64, 32, seed=97, noise=0.0)
+    unit = 2.0 ** (others + 7)
+    for rows in (case.key_rows, case.value_rows):
+        np.clip(rows, -4, 4, out=rows)
+        rows *= np.float32(unit)
+    np.clip(case.q, -4, 4, out=case.q)
+    case.q[:, ::64] = 4
+    case.scale = 0.125 / unit
+    channel = case.key_rows[..., 0]
+    channel[~np.isnan(channel)] = unit if first >= others else 60 * unit  # (scores of thirty)
+    pages = case.table[:, 0]
+    case.key_rows[pages, :, 0] = 0
+    case.value_rows[pages, :, 0] = 0
+    if first >= others:
+        case.key_rows[pages, :, 0, 0] = -300 * 2.0 ** first  # (a score of -150·2^(first - others - 7) and less)
+        case.value_rows[pages, :, 0] = 300 * 2.0 ** first
+    case.quantise()
+    got = attend(ctx, case)
+    want, _ = case.expected(True, np.full(got.shape, 7.25))
+    a = 0.125 * (4 * 60 + 63 * 16)
+    bound = 4 * unit * (2 * a * (72 * 2.0 ** -24 + 2.0 ** -22 + 2.0 ** -23) + 216 * 2.0 ** -24)
+    assert np.max(np.abs(want)) > unit / 8
+    assert np.max(np.abs(got - want)) <= bound
+
+
 @pytest.mark.parametrize("storage", STORAGES)
 @pytest.mark.parametrize("width", [64, 80, 128])
 @pytest.mark.parametrize("counts,lengths,kv", [([40, 4, 1], [40, 20, 77], 2), ([200], [300], 2), ([70, 1], [110, 40], 192)])
@@ -702,6 +735,17 @@ def test_empty_calls(ctx):
         ctx.paged_append(cache, rows, none, none)
         ctx.paged_read(cache, rows, none, none)
         ctx.paged_attention(cache, rows, none, 2, True, 0.125, none)
+    # Rows that see nothing: no length at all, and no table.
+    for lengths, table, longest in ((0, 4, 0), (0, 0, 9), (-5, 4, 9)):
+        y = torch.full((2, 128), 7.25, device="cuda")
+        nothing = PagedRows(torch.tensor([0, 1, 2], **i32), torch.full((2,), lengths, **i32),
+                            torch.zeros((2, table), **i32), 2, 1, longest)
+        ctx.paged_append(cache, nothing, y, y)
+        ctx.paged_attention(cache, nothing, y, 2, True, 0.125, y.clone())
+        out = torch.full((2, 128), 7.25, device="cuda")
+        ctx.paged_attention(cache, nothing, y, 2, False, 0.125, out)
+        torch.cuda.synchronize()
+        assert bool((out == 0).all())
     idle = PagedRows(torch.zeros(3, **i32), torch.full((2,), 9, **i32), torch.zeros((2, 4), **i32), 2, 1, 9)
     x = torch.full((2, 128), 7.25, device="cuda")
     ctx.paged_append(cache, idle, x, x)

@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
                 top = groups_max(top);
                 // 2^13 <= top·2^shift < 2^14 (a pair of zeros, or not finite: as it is)
                 int shift = 140 - (int) (__float_as_uint(top) >> 23);
-                shift = top > 0.f && top < INFINITY ? min(shift, 100) : 0;
+                shift = top > 0.f && top < INFINITY ? min(shift, 126) : 0;
 #pragma unroll
                 for (int i = 0; i < W / 4; ++i)
                     x[i] = ldexpf(x[i], shift);

@@ -66,6 +66,7 @@ __device__ __forceinline__ void lds_barrier()
 // ---------------------------------------------------------------------------
 constexpr int kChunkWaves = 4, kChunkKeys = 64;
 constexpr int kLeastShift = -15, kMostShift = 7;
+constexpr int kLeastBase = -7, kMostBase = 46; // rows' powers are 2^-80 to 2^120
 
 // The 16-byte run of run c of eight keys of a channel's row: eight consecutive
 // rows, and every fourth of 32, lie in different bank groups.
@@ -163,7 +164,7 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FU
         {
             // 2^13 <= top·2^shift < 2^14 (a pair of zeros, or not finite: as it is)
             top = halves_max(top);
-            shift = top > 0.f && top < INFINITY ? min(140 - (int) (__float_as_uint(top) >> 23), 100) : 0;
+            shift = top > 0.f && top < INFINITY ? min(140 - (int) (__float_as_uint(top) >> 23), 126) : 0;
             unit = ldexpf(1.f, -shift);
         }
 #pragma unroll
@@ -243,14 +244,18 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FU
                                                                              + (uint32_t) (4 * h));
     };
 
-    // E4M3: the powers that the operands leave out, those of the block's first rows.
+    // E4M3: the powers that the operands leave out, those of the first key's rows, or
+    // the nearest that keep every other row's within a float's range of them.
     int key_base = kExponentBias, value_base = kExponentBias;
     if (ST == kE4M3 && begin < end)
     {
         const int page = page_of(table, rows.table_width, cache.page_shift, cache.pages, begin);
         const size_t row = pool_row(max(page, 0), head, begin & page_mask, cache.heads, cache.page_shift);
-        key_base = cache.key_exponents[row];
-        value_base = cache.value_exponents[row];
+        auto base_of = [&](const uint8_t* exponents) {
+            return min(max((int) exponents[row], kExponentBias + kLeastBase), kExponentBias + kMostBase);
+        };
+        key_base = base_of(cache.key_exponents);
+        value_base = base_of(cache.value_exponents);
     }
     // 2^(byte - base) as a float's bits, for bytes within a float's range of the base.
     auto power_bits = [](uint32_t byte, int base) { return (byte + (uint32_t) (kExponentBias - base)) << 23; };

@@ -149,6 +149,7 @@ inline Plan plan_attention(const wsp_paged_cache& cache, const wsp_paged_rows& r
     if (splits < 2 || units > kSplitUnits || plan.tile_rows == kChunkRows)
         splits = 1;
     plan.span = (int) (((keys + splits - 1) / splits + 31) / 32 * 32);
+    plan.span = plan.span < 32 ? 32 : plan.span;
     plan.splits = splits == 1 ? 1 : (keys + plan.span - 1) / plan.span;
     return plan;
 }
