@@ -95,6 +95,10 @@ __device__ __forceinline__ void store_stored4(void* pool, size_t index, const fl
 // heads one after the other, all their loads in flight at once. The row's sequence,
 // position and page are the same for the wave, so the search and the addresses are
 // scalar. Append takes a head's largest magnitude over its lanes: a row is read once.
+// Bound by memory: 64k rows of eight E4M3 heads of 128 read back in 131 us, 5.1 TB/s (as
+// a large copy), up to 4096 rows of eight such sequences stored in 36, 4.4 TB/s; a step's
+// few rows by the launch (3.5 us). (Lanes that searched and divided for themselves, one
+// head each: 248 and 46 us.)
 // ---------------------------------------------------------------------------
 constexpr int kTurns = 4;
 

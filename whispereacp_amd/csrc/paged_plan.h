@@ -66,11 +66,6 @@ constexpr int shift_of(int page_rows)
     return shift;
 }
 
-constexpr size_t storage_bytes(int storage)
-{
-    return storage == WSP_F32 ? 4 : storage == WSP_E4M3 ? 1 : 2;
-}
-
 inline int say(char* why, size_t size, int code, const char* format, ...)
 {
     va_list args;
@@ -104,12 +99,15 @@ struct Plan
 };
 
 constexpr int kChunkRows = 128;   // of the kernel for many rows
-constexpr int kChunkBlocks = 384;
-constexpr int kRoundBlocks = 768; // blocks that run at once, three a CU
+constexpr int kChunkBlocks = 384; // from so many of its blocks on it is taken
+constexpr int kRoundBlocks = 768; // blocks of the other one that run at once, three a CU
 constexpr int kLeastSpan = 256;   // two turns of a block's waves
-constexpr int kMostSpan = 4096;   // lengths differ: blocks of longer spans end apart
-constexpr int kSplitUnits = 4096;  // counters, one for each row tile of a cached head
-constexpr int kJoinRows = 4096;    // partial rows that one block joins
+// Longer spans are cut even where the blocks already fill the chip: lengths differ. (64
+// sequences of up to 8192, eight cached heads of 128 in E4M3: 189 us in spans of 1024,
+// 162 of 2048, 150 of 4096, where a block's start and its hand-over weigh least.)
+constexpr int kMostSpan = 4096;
+constexpr int kSplitUnits = 4096; // counters, one for each row tile of a cached head
+constexpr int kJoinRows = 4096;   // partial rows that one block joins
 // Splits that the last block of a row tile joins itself; more are joined by a launch
 // of their own (one token over 131072 positions, 96 splits: 110 us so, 124 by the last
 // block; four tokens over 1500 of 16 streams, three splits: 25 and 23.5).
