@@ -168,9 +168,9 @@ int main()
 
     // Plans: what the launches index fits the scratch, the counters, the join's factors
     // and a launch's extents, and the splits cover every key a row can see.
-    const size_t scratch = (16 << 20) / sizeof(float);
+    const size_t scratch = kPartialBytes / sizeof(float);
     right = true;
-    int split = 0, chunked = 0;
+    int split = 0, chunked = 0, cut_chunks = 0;
     for (int storage = WSP_F32; storage <= WSP_E4M3; ++storage)
         for (int width : {16, 64, 80, 128})
             for (int heads : {1, 6, 20, 200, 5000})
@@ -200,16 +200,16 @@ int main()
                                     ++split;
                                     right = right
                                             && (unsigned long long) units * p.splits * p.row_slots * (width + 2) <= scratch
-                                            && units <= kSplitUnits && p.splits * p.row_slots <= kJoinRows
+                                            && (!p.fused || (units <= kSplitUnits && p.splits * p.row_slots <= kJoinRows))
                                             && p.row_slots >= std::min<long long>(pairs, p.tile_rows)
-                                            && p.span % 32 == 0
-                                            && (long long) p.span * p.splits >= key_bound(r, c.page_rows)
-                                            && p.tile_rows != kChunkRows;
+                                            && p.span % 64 == 0
+                                            && (long long) p.span * p.splits >= key_bound(r, c.page_rows);
+                                    cut_chunks += p.tile_rows == kChunkRows;
                                 }
                                 chunked += p.tile_rows == kChunkRows;
                                 right = right && (storage != WSP_F32 || p.tile_rows != kChunkRows);
                             }
-    expect(right && split > 100 && chunked > 100, "plans fit what they index");
+    expect(right && split > 100 && chunked > 100 && cut_chunks > 20, "plans fit what they index");
     wsp_paged_rows table_rows = good_rows(); // 2 pages of 16
     table_rows.max_length = 1000;
     expect(key_bound(table_rows, 16) == 33, "a row that sees past the table sees one key there");

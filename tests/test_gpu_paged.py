@@ -399,7 +399,7 @@ CHUNKS = [
     # counts, lengths, kv, group, width, page, spare rows
     ([70, 0, 66], [70, 9, 300], 192, 1, 64, 16, 2),
     ([65, 3], [200, 3], 192, 1, 128, 32, 0),
-    ([40, 129], [90, 130], 64, 3, 96, 64, 1),                       # shared heads, a ragged last tile
+    ([40, 129], [90, 130], 96, 3, 96, 64, 1),                       # shared heads, a ragged last tile
     ([33, 1], [64, 700], 200, 2, 48, 16, 0),                        # narrow heads
     ([90, 20], [500, 20], 200, 1, 112, 16, 0),
     ([100, 80], [64, 81], 200, 1, 80, 128, 0),                      # rows before their sequence
@@ -413,6 +413,14 @@ def test_attention_of_chunks(ctx, storage, causal, counts, lengths, kv, group, w
     check(ctx, Case(storage, counts, lengths, kv, group, width, page, seed=83, spare_rows=spare), causal)
 
 
+@pytest.mark.parametrize("storage", ["F16", "BF16", "E4M3"])
+@pytest.mark.parametrize("kv,width", [(96, 64), (64, 80), (64, 128)])
+def test_attention_of_chunks_over_long_sequences(ctx, storage, kv, width):
+    # The 128-row kernel with its keys cut: the second sequence ends in the first cut,
+    # rows of the first end on either side of it.
+    check(ctx, Case(storage, [129, 70], [4160, 100], kv, 1, width, 64, seed=101))
+
+
 @pytest.mark.parametrize("storage", STORAGES)
 @pytest.mark.parametrize("count,length", [(1, 5000), (3, 9000), (20, 4100)])
 def test_attention_over_long_sequences(ctx, storage, count, length):
@@ -422,7 +430,7 @@ def test_attention_over_long_sequences(ctx, storage, count, length):
 
 @pytest.mark.parametrize("storage", STORAGES)
 @pytest.mark.parametrize("width", [64, 128])
-@pytest.mark.parametrize("kv", [1, 128])
+@pytest.mark.parametrize("kv", [1, 192])
 def test_attention_of_large_scores(ctx, storage, width, kv):
     # Scores of some hundreds: one key takes nearly all, the running maximum
     # climbs along the keys, and late keys push early ones out.
@@ -437,7 +445,7 @@ def test_attention_of_large_scores(ctx, storage, width, kv):
 
 @pytest.mark.parametrize("storage", ["F16", "BF16", "E4M3", "F32"])
 @pytest.mark.parametrize("q_size,v_size", [(1e-6, 1e4), (1e5, 1e-4), (0.0, 1.0)])
-@pytest.mark.parametrize("kv", [2, 128])
+@pytest.mark.parametrize("kv", [2, 192])
 def test_attention_of_odd_magnitudes(ctx, storage, q_size, v_size, kv):
     # Queries far from one (their parts are scaled to fp16's range), values large
     # and small. Scores stay ordinary: scale undoes the queries' size.
@@ -673,7 +681,7 @@ def test_a_prompt_and_steps_together(ctx, storage):
 
 
 def test_the_same_bits_every_time(ctx):
-    for count, kv in ((1, 2), (7, 2), (64, 2), (64, 96)):
+    for count, kv in ((1, 2), (7, 2), (64, 2), (64, 192)):
         case = Case("E4M3", [count, count], [2000, 700], kv, 2, 128, 64, seed=71)
         cache, rows = case.cache(), case.packed()
         first = attend(ctx, case, cache=cache, rows=rows)

@@ -92,14 +92,15 @@ int wsp_hip_ctx_create(const wsp_decoder_shape* shape, int device, void* stream,
         ctx->parts_bytes = std::max<size_t>(
             16 << 20, wsp::ops::parts_bytes((size_t) longest * std::max(shape->width, shape->feed_forward_width)));
         // One block: the attention workspace, the argmax candidates, the paged
-        // attention's counters, the parts.
+        // attention's counters, the parts, the paged attention's partial rows.
         auto rounded = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
         const size_t attention = rounded(std::max(ctx->attention_floats, wsp::ops::kQueryAttentionFloats)
                                          * sizeof(float));
         const size_t candidates = rounded(ctx->argmax_candidates * sizeof(float));
         const size_t counters = rounded(wsp::paged::kSplitUnits * sizeof(unsigned int));
         char* block = nullptr;
-        status = hip_status(ctx, hipMalloc(&block, attention + 2 * candidates + counters + ctx->parts_bytes),
+        status = hip_status(ctx, hipMalloc(&block, attention + 2 * candidates + counters
+                                                       + rounded(ctx->parts_bytes) + wsp::paged::kPartialBytes),
                             "workspace");
         if (status == WSP_OK)
         {
@@ -108,6 +109,7 @@ int wsp_hip_ctx_create(const wsp_decoder_shape* shape, int device, void* stream,
             ctx->argmax_indices = reinterpret_cast<uint32_t*>(block + attention + candidates);
             ctx->paged_counters = reinterpret_cast<unsigned int*>(block + attention + 2 * candidates);
             ctx->parts = block + attention + 2 * candidates + counters;
+            ctx->paged_partials = block + attention + 2 * candidates + counters + rounded(ctx->parts_bytes);
             // The prompt attention's per-head counters start at zero (each launch
             // leaves them zero again).
             status = hip_status(ctx, hipMemset(ctx->attention_workspace, 0,

@@ -26,7 +26,10 @@ struct wsp_hip_ctx
     void* parts = nullptr;
     size_t parts_bytes = 0;
 
-    unsigned int* paged_counters = nullptr; // paged::kSplitUnits, zero between calls
+    // The paged attention's partial rows (paged::kPartialBytes), and its counters
+    // (paged::kSplitUnits, zero between calls).
+    void* paged_partials = nullptr;
+    unsigned int* paged_counters = nullptr;
 
     void* fused = nullptr; // fused-step state (fused_step.hip)
 

@@ -187,7 +187,7 @@ __device__ __forceinline__ void load_words(const char* at, uint32_t (&words)[WOR
 }
 
 // One launch over row tiles first_tile on and sequences first_sequence on (its
-// grid: heads, tiles, sequences), by the kernel for many rows (paged_chunk.hip).
+// grid: splits·heads, tiles, sequences), by the kernel for many rows (paged_chunk.hip).
 void launch_chunks(hipStream_t stream, dim3 grid, int storage, const Cache& cache, const Rows& rows,
-                   const Query& query, int first_tile, int first_sequence);
+                   const Query& query, const Split& split, int first_tile, int first_sequence);
 } // namespace wsp::paged

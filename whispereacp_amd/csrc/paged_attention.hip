@@ -763,6 +763,58 @@ __global__ void __launch_bounds__(kJoinWaves* kWave) join_kernel(Cache cache, Ro
     }
 }
 
+// The same for few splits of many rows: a wave for each row.
+__global__ void __launch_bounds__(kJoinWaves* kWave) join_few_kernel(Cache cache, Rows rows, Query query, Split split,
+                                                                     int tile_rows, int first_tile, int first_sequence)
+{
+    const int groups = (split.row_slots + kJoinWaves - 1) / kJoinWaves;
+    const int slot = blockIdx.x % groups * kJoinWaves + threadIdx.x / kWave, head = blockIdx.x / groups;
+    RowTile tl;
+    if (!find_tile(rows, query, first_sequence + blockIdx.z, first_tile + (int) (gridDim.y - 1 - blockIdx.y), tile_rows,
+                   tl))
+        return;
+    const int pair = tl.first + slot, used = splits_used(tl, split.span);
+    if (pair > tl.last || used == 1)
+        return;
+    const int width = cache.head_width, lane = threadIdx.x % kWave;
+    const int unit = ((int) blockIdx.z * (int) gridDim.y + (int) blockIdx.y) * cache.heads + head;
+    const float* first = partial_row(split, unit, 0, slot, width);
+    const size_t pitch = (size_t) split.row_slots * (width + 2);
+    // Lane i holds split i's maximum and sum (a split without a key of finite score
+    // sums to zero).
+    const int own = min(lane, used - 1);
+    const float top = first[own * pitch], sum = lane < used ? first[own * pitch + 1] : 0.f;
+    const float factor = sum == 0.f ? 0.f : __builtin_amdgcn_exp2f(top - wave_max(lane < used ? top : -INFINITY));
+    const float total = wave_sum(factor * sum);
+    const int c0 = min(lane, width - 1), c1 = min(lane + kWave, width - 1);
+    float low = 0.f, high = 0.f;
+    constexpr int kAtOnce = 4;
+    for (int i0 = 0; i0 < used; i0 += kAtOnce)
+    {
+        float a[kAtOnce], b[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+        {
+            const float* part = first + min(i0 + i, used - 1) * pitch + 2;
+            a[i] = part[c0];
+            b[i] = part[c1];
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+        {
+            const float f = i0 + i < used ? __shfl(factor, i0 + i) : 0.f;
+            low += f == 0.f ? 0.f : f * a[i];
+            high += f == 0.f ? 0.f : f * b[i];
+        }
+    }
+    float* const out = out_of(tl, query, head, pair, width, 0);
+    if (lane < width)
+        out[lane] = total == 0.f ? 0.f : low / total;
+    if (lane + kWave < width)
+        out[lane + kWave] = total == 0.f ? 0.f : high / total;
+}
+static_assert(kFusedSplits <= kWave, "a lane for each split");
+
 constexpr int kMostBlocks = 65535; // of a launch's y and z extents
 
 void launch_tiles(hipStream_t stream, dim3 grid, int storage, const Cache& cache, const Rows& rows,
@@ -799,7 +851,7 @@ hipError_t attention(hipStream_t stream, const wsp_paged_cache& cache, const wsp
     const Query query {q, q_stride, heads, heads / cache.heads, causal, scale * 1.4426950408889634f, out, out_stride};
     const Plan plan = plan_attention(cache, rows, query.group, scratch.bytes / sizeof(float));
     const Split split {plan.splits, plan.span, plan.row_slots, static_cast<float*>(scratch.data),
-                       plan.splits > kFusedSplits ? nullptr : scratch.counters};
+                       plan.fused ? scratch.counters : nullptr};
     const Cache pool = device_cache(cache);
     const Rows packed = device_rows(cache, rows);
     for (int s = 0; s < rows.sequences; s += plan.slice)
@@ -808,12 +860,15 @@ hipError_t attention(hipStream_t stream, const wsp_paged_cache& cache, const wsp
             const dim3 grid(split.splits * cache.heads, std::min(plan.tiles - t, kMostBlocks),
                             std::min(rows.sequences - s, plan.slice));
             if (plan.tile_rows == kChunkRows)
-                launch_chunks(stream, grid, cache.storage, pool, packed, query, t, s);
+                launch_chunks(stream, grid, cache.storage, pool, packed, query, split, t, s);
             else
                 launch_tiles(stream, grid, cache.storage, pool, packed, query, split, plan.tile_rows, t, s);
             if (split.splits > kFusedSplits)
                 join_kernel<<<dim3(cache.heads * split.row_slots, grid.y, grid.z), kJoinWaves * kWave, 0, stream>>>(
                     pool, packed, query, split, plan.tile_rows, t, s);
+            else if (split.splits > 1 && !plan.fused)
+                join_few_kernel<<<dim3(cache.heads * ((split.row_slots + kJoinWaves - 1) / kJoinWaves), grid.y, grid.z),
+                                  kJoinWaves * kWave, 0, stream>>>(pool, packed, query, split, plan.tile_rows, t, s);
         }
     return hipGetLastError();
 }

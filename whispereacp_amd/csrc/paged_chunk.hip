@@ -44,8 +44,8 @@ __device__ __forceinline__ void lds_barrier()
 
 // ---------------------------------------------------------------------------
 // Many rows: attention of a tile of 128 pairs (new row, head of the group), 32 a
-// wave, over the keys of one cached head, 64 at a time through LDS. The block
-// converts and transposes what the storage holds once for its 128 pairs: keys as
+// wave, over keys [split·span, +span) of one cached head, 64 at a time through LDS. The
+// block converts and transposes what the storage holds once for its 128 pairs: keys as
 // [key][channel], values as [channel][key], 16-bit operands of v_mfma_f32_32x32x16.
 //
 // S^T = K·Q^T leaves lane (n, h) with keys 8i + 4h + r (i, r < 4) of each 32 and
@@ -107,7 +107,7 @@ constexpr int kChunkOccupancy = (ST == kBF16 && C >= 96) || (!FULL && C == 128) 
 // 32); FULL: the heads are C wide.
 template <int ST, int W, int C, bool FULL>
 __global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FULL>))
-    chunk_attention_kernel(Cache cache, Rows rows, Query query, int first_tile, int first_sequence)
+    chunk_attention_kernel(Cache cache, Rows rows, Query query, Split split, int first_tile, int first_sequence)
 {
     constexpr int OT = operand_of<ST>, kParts = parts_of<OT>();
     constexpr float kBias = OT == kF16 ? 14.f : 0.f;
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FU
     // and the last E4M3 one whose rows' powers are not in the operands.
     __shared__ int odd_tile, apart_tile;
 
-    const int head = blockIdx.x;
+    const int which = blockIdx.x % split.splits, head = blockIdx.x / split.splits;
     const int sequence = first_sequence + blockIdx.z;
     const int tile = first_tile + (int) (gridDim.y - 1 - blockIdx.y); // (the tiles that see most come first)
     RowTile tl;
@@ -134,9 +134,10 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FU
     const int width = FULL ? C : cache.head_width, row_bytes = width * bytes_of<ST>;
     const int page_mask = (1 << cache.page_shift) - 1;
     const int* table = rows.pages + (size_t) sequence * rows.table_width;
-    const int end = tl.poisoned ? 0 : tl.most;
-    int begin = 0; // (opaque: with the constant the loop's first turn gets code, and registers, of its own)
-    asm("" : "+s"(begin));
+    const int used = splits_used(tl, split.span);
+    if (which >= used)
+        return;
+    const int begin = which * split.span, end = tl.poisoned ? 0 : min(begin + split.span, tl.most);
 
     // This wave's pairs: lane (n, h) holds channels 16j + 8h .. + 7 of pair n.
     const int first = tl.first + 32 * wave, pair = first + n;
@@ -591,8 +592,15 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FU
     if (!real)
         return;
     const float power = ldexpf(1.f, value_base - kExponentBias);
-    const float by = l == 0.f ? 0.f : power / l;
-    float* const out = out_of(tl, query, head, pair, width, 0);
+    const float by = used > 1 ? power : l == 0.f ? 0.f : power / l;
+    const int unit_index = ((int) blockIdx.z * (int) gridDim.y + (int) blockIdx.y) * cache.heads + head;
+    float* const part = partial_row(split, unit_index, which, pair - tl.first, width);
+    float* const out = used > 1 ? part + 2 : out_of(tl, query, head, pair, width, 0);
+    if (used > 1 && h == 0)
+    {
+        part[0] = m;
+        part[1] = l;
+    }
 #pragma unroll
     for (int c = 0; c < C / 32; ++c)
 #pragma unroll
@@ -604,13 +612,13 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FU
 } // namespace
 
 void launch_chunks(hipStream_t stream, dim3 grid, int storage, const Cache& cache, const Rows& rows,
-                   const Query& query, int first_tile, int first_sequence)
+                   const Query& query, const Split& split, int first_tile, int first_sequence)
 {
     by_storage(storage, [&](auto type) {
         auto run = [&](auto width, auto channels, auto full) {
             if constexpr (type() != kF32)
                 chunk_attention_kernel<type(), width(), channels(), full()><<<grid, kChunkWaves * kWave, 0, stream>>>(
-                    cache, rows, query, first_tile, first_sequence);
+                    cache, rows, query, split, first_tile, first_sequence);
         };
         using Narrow = std::integral_constant<int, 64>;
         using Middle = std::integral_constant<int, 96>;

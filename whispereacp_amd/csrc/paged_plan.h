@@ -6,6 +6,7 @@
 
 #include "../../include/wsp_hip.h"
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstddef>
 #include <cstdint>
@@ -95,12 +96,14 @@ struct Plan
 {
     int tile_rows, tiles;
     int splits, span, row_slots;
+    bool fused; // the splits are joined by the last block of their tile
     int slice;
 };
 
 constexpr int kChunkRows = 128;   // of the kernel for many rows
 constexpr int kChunkBlocks = 384; // from so many of its blocks on it is taken
-constexpr int kRoundBlocks = 768; // blocks of the other one that run at once, three a CU
+constexpr int kChunkSpan = 2048;  // least keys of a cut (4096 pairs over 30000 keys of 8 heads of 64: 980 us uncut, 724 in three)
+constexpr int kRoundBlocks = 768; // blocks that run at once, three a CU
 constexpr int kLeastSpan = 256;   // two turns of a block's waves
 // Longer spans are cut even where the blocks already fill the chip: lengths differ. (64
 // sequences of up to 8192, eight cached heads of 128 in E4M3: 189 us in spans of 1024,
@@ -108,11 +111,12 @@ constexpr int kLeastSpan = 256;   // two turns of a block's waves
 constexpr int kMostSpan = 4096;
 constexpr int kSplitUnits = 4096; // counters, one for each row tile of a cached head
 constexpr int kJoinRows = 4096;   // partial rows that one block joins
-// Splits that the last block of a row tile joins itself; more are joined by a launch
-// of their own (one token over 131072 positions, 96 splits: 110 us so, 124 by the last
+// Splits that the last block of a tile of few rows joins itself; more, and those of many
+// rows, are joined by a launch of their own (one token over 131072 positions, 96 splits: 110 us so, 124 by the last
 // block; four tokens over 1500 of 16 streams, three splits: 25 and 23.5).
 constexpr int kFusedSplits = 16;
 constexpr int kMostSequences = 65535; // a launch's z extent
+constexpr size_t kPartialBytes = (size_t) 64 << 20; // a context's room for partial rows
 
 inline Plan plan_attention(const wsp_paged_cache& cache, const wsp_paged_rows& rows, int group, size_t scratch_floats)
 {
@@ -120,20 +124,39 @@ inline Plan plan_attention(const wsp_paged_cache& cache, const wsp_paged_rows& r
     const int storage = cache.storage, heads = cache.heads, head_width = cache.head_width;
     const long long pairs = (long long) (rows.max_count < rows.rows ? rows.max_count : rows.rows) * group;
     const int keys = key_bound(rows, cache.page_rows);
-    // Blocks of 128 rows where they make a round and a half of the chip: each takes
-    // longer (16 sequences of 512 rows over 2048 keys of 12 heads of 64, fp16: 128 us and 176
-    // in blocks of 32; 4 sequences 87 and 55; 64 of 32 rows over 4096, heads of 128 in
-    // E4M3, 237 and 147 in blocks of 16).
-    const long long chunks = (pairs + kChunkRows - 1) / kChunkRows * heads * rows.sequences;
-    if (storage != WSP_F32 && pairs > kChunkRows / 2 && chunks >= kChunkBlocks)
+    plan.slice = rows.sequences < kMostSequences ? rows.sequences : kMostSequences;
+    auto per_unit = [&](int slots) { return (size_t) slots * (head_width + 2); };
+    auto held = [&](long long units, int slots) { // splits whose partial rows the scratch holds
+        return (long long) (scratch_floats / per_unit(slots) / units);
+    };
+    // Blocks of 128 rows where they, cut along long keys, make a round and a half of the
+    // chip: each takes longer than smaller ones, and more of it lies idle behind a
+    // sequence's last row. 512 rows over 2048 keys of 12 heads of 64, fp16, 16 sequences:
+    // 128 us and 176 in blocks of 32, 8 sequences 97 and 95, 4 sequences 87 and 55; heads
+    // of 128, 261 and 412 in blocks of 16, 139 and 213, 107 and 114. 14 sequences of up to
+    // 333 rows over up to 13554 bf16 keys of 14 heads of 64, 656 and 420. (The packed rows
+    // tell how many blocks there are at most, but for half a block a sequence.)
+    const long long chunks = (pairs + kChunkRows - 1) / kChunkRows * heads * plan.slice;
+    const long long filled =
+        ((long long) rows.rows * group / kChunkRows + rows.sequences / 2 + 1) * heads; // about
+    long long chunk_splits = kRoundBlocks / chunks;
+    if (chunks < kRoundBlocks / 3 && chunk_splits < keys / kMostSpan) // (four sequences of up to 54000
+        chunk_splits = keys / kMostSpan;                              // keys: 489 us in 7, 363 in 13)
+    if (chunk_splits > kFusedSplits)
+        chunk_splits = kFusedSplits;
+    if (chunk_splits > keys / kChunkSpan)
+        chunk_splits = keys / kChunkSpan;
+    if (chunk_splits > held(chunks, kChunkRows))
+        chunk_splits = held(chunks, kChunkRows);
+    if (chunk_splits < 1)
+        chunk_splits = 1;
+    if (storage != WSP_F32 && pairs > kChunkRows / 2 && std::min(chunks, filled) * chunk_splits >= kChunkBlocks)
         plan.tile_rows = kChunkRows;
     else
         plan.tile_rows = pairs <= 16 || head_width > 64 ? 16 : 32;
     plan.tiles = (int) ((pairs + plan.tile_rows - 1) / plan.tile_rows);
     plan.row_slots = (int) (pairs < plan.tile_rows ? pairs : plan.tile_rows);
-    plan.slice = rows.sequences < kMostSequences ? rows.sequences : kMostSequences;
     const long long units = (long long) plan.tiles * heads * plan.slice;
-    const size_t unit_floats = (size_t) plan.row_slots * (head_width + 2);
     // As many splits as still run at once, or as keep the spans short.
     long long splits = (keys + kLeastSpan - 1) / kLeastSpan;
     if (splits > kRoundBlocks / units)
@@ -142,13 +165,16 @@ inline Plan plan_attention(const wsp_paged_cache& cache, const wsp_paged_rows& r
         splits = (keys + kMostSpan - 1) / kMostSpan;
     if (splits > kJoinRows / plan.row_slots)
         splits = kJoinRows / plan.row_slots;
-    if ((unsigned long long) splits > scratch_floats / unit_floats / units)
-        splits = (long long) (scratch_floats / unit_floats / units);
-    if (splits < 2 || units > kSplitUnits || plan.tile_rows == kChunkRows)
+    if (splits > held(units, plan.row_slots))
+        splits = held(units, plan.row_slots);
+    if (splits < 2 || units > kSplitUnits)
         splits = 1;
-    plan.span = (int) (((keys + splits - 1) / splits + 31) / 32 * 32);
-    plan.span = plan.span < 32 ? 32 : plan.span;
+    if (plan.tile_rows == kChunkRows)
+        splits = chunk_splits;
+    plan.span = (int) (((keys + splits - 1) / splits + 63) / 64 * 64);
+    plan.span = plan.span < 64 ? 64 : plan.span;
     plan.splits = splits == 1 ? 1 : (keys + plan.span - 1) / plan.span;
+    plan.fused = plan.splits <= kFusedSplits && plan.tile_rows != kChunkRows;
     return plan;
 }
 
