@@ -65,7 +65,7 @@ __device__ __forceinline__ void lds_barrier()
 // work. Bound by both together: two chunks of 2048 rows over 16384 E4M3 positions (32
 // query heads over eight, heads of 128) take 2.0 to 2.2 ms, 0.5 PFLOP/s of the
 // algorithm and twice that in two-part products, of the 1.08 an 8192-cubed fp16 library
-// product reaches; the matrix cores are busy 43% of the time, the vector units 48%,
+// product reaches; the matrix cores are busy 44% of the time, the vector units 47%,
 // seldom at once. (Eight waves a block, each over half the keys: 2.6 ms, with two tiles
 // in LDS 3.6, its spills waiting for the loads in flight.) The accumulators are the
 // matrix cores' own through all keys: 1.2·10^-6 off in that case, 4·10^-7 where every 32
