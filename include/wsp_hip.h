@@ -70,9 +70,10 @@ typedef struct wsp_hip_ctx wsp_hip_ctx;
  * default stream) and sizes its workspaces for `shape` (attention partials,
  * argmax candidates, and the 16-bit parts of a product's rows: six bytes for
  * each value of the longest input over the widest layer, 46 MB at large-v3 and
- * 16 MB at least; 64 MB of the paged attention's partial rows). Replaces KernelNet::prepare's scratch and the
- * SingleQueryAttention/Argmax prepare() sizing (Net/KernelNet.cpp:133-207,
- * Kernels/SingleQueryAttention.cpp:32-60, Kernels/Argmax.cpp:26-40). */
+ * 16 MB at least; 64 MB for the paged attention's partial rows). Replaces
+ * KernelNet::prepare's scratch and the SingleQueryAttention/Argmax prepare()
+ * sizing (Net/KernelNet.cpp:133-207, Kernels/SingleQueryAttention.cpp:32-60,
+ * Kernels/Argmax.cpp:26-40). */
 int wsp_hip_ctx_create(const wsp_decoder_shape* shape, int device, void* stream,
                        wsp_hip_ctx** out);
 void wsp_hip_ctx_destroy(wsp_hip_ctx* ctx);
@@ -236,8 +237,9 @@ int wsp_hip_paged_read(wsp_hip_ctx* ctx, const wsp_paged_cache* cache, const wsp
  * others every position before lengths[s]. heads is a multiple of the cache's
  * heads; query head h reads cache head h / (heads / cache heads). scale
  * multiplies the summed dot product. A row that sees no key gets zeros; keys and
- * values that a row does not see do not reach it, whatever they hold. (One that
- * sees an infinity or NaN in a key is NaN, in F32 storage as fp32 has it.) */
+ * values that a row does not see do not reach it, whatever they hold. (A row that
+ * sees an infinity or NaN in a key is NaN, in F32 storage as fp32 has it; in a
+ * value, not finite in that channel.) */
 int wsp_hip_paged_attention(wsp_hip_ctx* ctx, const wsp_paged_cache* cache, const wsp_paged_rows* rows,
                             const float* q, int q_stride, int heads, int causal, float scale, float* out,
                             int out_stride);

@@ -800,5 +800,7 @@ def test_refusals(ctx):
     i32 = dict(dtype=torch.int32, device="cuda")
     with pytest.raises(ValueError, match="int32"):
         PagedRows(torch.zeros(2, device="cuda"), torch.zeros(1, **i32), torch.zeros((1, 1), **i32), 1, 1, 1)
+    with pytest.raises(ValueError, match="positions a sequence"):
+        PagedRows(torch.zeros(2, **i32), torch.zeros(1, **i32), torch.zeros((1, 1), **i32), 2 ** 32, 1, 1)
     with pytest.raises(ValueError, match="sequences"):
         PagedRows(torch.zeros(3, **i32), torch.zeros(1, **i32), torch.zeros((1, 1), **i32), 1, 1, 1)

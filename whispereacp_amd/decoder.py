@@ -103,28 +103,34 @@ class KernelContext:
     def paged_append(self, cache, rows, keys, values):
         """Stores the packed rows keys and values [rows.rows, heads·head_width] in
         their sequences' pages (paged.PagedCache, paged.PagedRows)."""
-        rows.check(cache, self.device)
-        width = cache.heads * cache.head_width
-        self._check(self.lib.wsp_hip_paged_append(
-            self.handle, cache.table, rows.table, ptr(keys), rows.stride(keys, width, self.device), ptr(values),
-            rows.stride(values, width, self.device)))
+        device, width = self.device, cache.width
+        rows.check(cache, device)
+        status = self.lib.wsp_hip_paged_append(
+            self.handle, cache.table, rows.table, keys.data_ptr(), rows.stride(keys, width, device), values.data_ptr(),
+            rows.stride(values, width, device))
+        if status:
+            self._check(status)
 
     def paged_read(self, cache, rows, keys, values):
         """Writes the packed rows' stored values to keys and values, fp32."""
-        rows.check(cache, self.device)
-        width = cache.heads * cache.head_width
-        self._check(self.lib.wsp_hip_paged_read(
-            self.handle, cache.table, rows.table, ptr(keys), rows.stride(keys, width, self.device), ptr(values),
-            rows.stride(values, width, self.device)))
+        device, width = self.device, cache.width
+        rows.check(cache, device)
+        status = self.lib.wsp_hip_paged_read(
+            self.handle, cache.table, rows.table, keys.data_ptr(), rows.stride(keys, width, device), values.data_ptr(),
+            rows.stride(values, width, device))
+        if status:
+            self._check(status)
 
     def paged_attention(self, cache, rows, q, heads, causal, scale, out):
         """Attention of the packed rows q [rows.rows, heads·head_width] over their
         sequences' pages, into out."""
-        rows.check(cache, self.device)
-        width = heads * cache.head_width
-        self._check(self.lib.wsp_hip_paged_attention(
-            self.handle, cache.table, rows.table, ptr(q), rows.stride(q, width, self.device), heads, int(causal), scale,
-            ptr(out), rows.stride(out, width, self.device)))
+        device, width = self.device, heads * cache.head_width
+        rows.check(cache, device)
+        status = self.lib.wsp_hip_paged_attention(
+            self.handle, cache.table, rows.table, q.data_ptr(), rows.stride(q, width, device), heads, int(causal), scale,
+            out.data_ptr(), rows.stride(out, width, device))
+        if status:
+            self._check(status)
 
     def argmax(self, logits, rows, row_length, mask, out):
         self._check(self.lib.wsp_hip_argmax(self.handle, ptr(logits), rows, row_length, ptr(mask), ptr(out)))

@@ -30,6 +30,7 @@ _CODES = {dtype: code for code, dtype in STORAGES.values()}
 
 
 _FLOAT = torch.float32
+_MOST = 2 ** 31 - 1  # of an extent
 
 
 class PagedCache:
@@ -56,6 +57,7 @@ class PagedCache:
             raise ValueError("the pool's tensors lie on one device")
         self.keys, self.values, self.key_exponents, self.value_exponents = keys, values, key_exponents, value_exponents
         self.pages, self.heads, self.page_rows, self.head_width = keys.shape
+        self.width = self.heads * self.head_width  # of a packed row
         self.device = keys.get_device()  # -1: not a GPU's
         self._ctable = N.wsp_paged_cache(_CODES[keys.dtype], self.pages, self.page_rows, self.heads, self.head_width,
                                          keys.data_ptr(), values.data_ptr(),
@@ -93,6 +95,8 @@ class PagedRows:
             raise ValueError("starts is [sequences + 1], lengths [sequences] and the table [sequences, table_width]")
         if len({t.device for t in self._keep}) != 1:
             raise ValueError("starts, lengths and the table lie on one device")
+        if not all(0 <= n <= _MOST for n in (rows, max_count, max_length, table.shape[1])):
+            raise ValueError(f"{rows} rows, at most {max_count} of {max_length} positions a sequence")
         self.rows = rows
         self.device = lengths.get_device()
         self._ctable = N.wsp_paged_rows(sequences, rows, max_count, max_length, table.shape[1], starts.data_ptr(),
@@ -110,4 +114,7 @@ class PagedRows:
             raise ValueError(f"packed rows are fp32 [{self.rows}, {width}], each row in one run")
         if tensor.get_device() != device:
             raise ValueError(f"a tensor on {tensor.device} for a context on device {device}")
-        return strides[0] if shape[0] > 1 else max(width, strides[0])
+        apart = strides[0] if shape[0] > 1 else width
+        if apart > _MOST:
+            raise ValueError(f"packed rows {apart} floats apart (at most {_MOST})")
+        return apart
