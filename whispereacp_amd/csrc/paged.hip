@@ -137,9 +137,9 @@ __device__ __forceinline__ Place place_of(const Cache& cache, const Rows& rows, 
 }
 
 template <int ST, int LANES>
-__global__ void __launch_bounds__(kBlock) append_kernel(Cache cache, Rows rows, int first_row, const float* __restrict__ keys,
-                                                        int key_stride, const float* __restrict__ values,
-                                                        int value_stride)
+__global__ void __launch_bounds__(kBlock)
+    append_kernel(Cache cache, Rows rows, int first_row, const float* __restrict__ keys, int key_stride,
+                  const float* __restrict__ values, int value_stride)
 {
     const int row = first_row + (int) blockIdx.x * kWavesPerBlock + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const Place at = place_of(cache, rows, row);
@@ -195,8 +195,9 @@ __global__ void __launch_bounds__(kBlock) append_kernel(Cache cache, Rows rows, 
 }
 
 template <int ST, int LANES>
-__global__ void __launch_bounds__(kBlock) read_kernel(Cache cache, Rows rows, int first_row, float* __restrict__ keys,
-                                                      int key_stride, float* __restrict__ values, int value_stride)
+__global__ void __launch_bounds__(kBlock)
+    read_kernel(Cache cache, Rows rows, int first_row, float* __restrict__ keys, int key_stride,
+                float* __restrict__ values, int value_stride)
 {
     const int row = first_row + (int) blockIdx.x * kWavesPerBlock + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const Place at = place_of(cache, rows, row);

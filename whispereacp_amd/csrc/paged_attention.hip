@@ -173,9 +173,8 @@ template <int ST, int W, int QT>
 constexpr int kTileOccupancy = QT == 1 && W == 64 && ST != kF32 ? 3 : 2;
 
 template <int ST, int W, bool FULL, int QT>
-__global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)) tile_attention_kernel(Cache cache, Rows rows, Query query,
-                                                                              Split split, int first_tile,
-                                                                              int first_sequence)
+__global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>))
+    tile_attention_kernel(Cache cache, Rows rows, Query query, Split split, int first_tile, int first_sequence)
 {
     constexpr int OT = operand_of<ST>, kParts = parts_of<OT>(), kWaves = kTileWaves, CPL = W / 16;
     constexpr float kBias = OT == kF16 ? 14.f : 0.f; // the weights' exponent (see above)

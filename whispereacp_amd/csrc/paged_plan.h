@@ -102,7 +102,9 @@ struct Plan
 
 constexpr int kChunkRows = 128;   // of the kernel for many rows
 constexpr int kChunkBlocks = 384; // from so many of its blocks on it is taken
-constexpr int kChunkSpan = 2048;  // least keys of a cut (4096 pairs over 30000 keys of 8 heads of 64: 980 us uncut, 724 in three)
+// Least keys of a cut of its (4096 pairs over 30000 keys of 8 heads of 64: 980 us
+// uncut, 724 in three).
+constexpr int kChunkSpan = 2048;
 constexpr int kRoundBlocks = 768; // blocks that run at once, three a CU
 constexpr int kLeastSpan = 256;   // two turns of a block's waves
 // Longer spans are cut even where the blocks already fill the chip: lengths differ. (64
@@ -112,8 +114,9 @@ constexpr int kMostSpan = 4096;
 constexpr int kSplitUnits = 4096; // counters, one for each row tile of a cached head
 constexpr int kJoinRows = 4096;   // partial rows that one block joins
 // Splits that the last block of a tile of few rows joins itself; more, and those of many
-// rows, are joined by a launch of their own (one token over 131072 positions, 96 splits: 110 us so, 124 by the last
-// block; four tokens over 1500 of 16 streams, three splits: 25 and 23.5).
+// rows, are joined by a launch of their own (one token over 131072 positions, 96 splits:
+// 110 us so, 124 by the last block; four tokens over 1500 of 16 streams, three splits: 25
+// and 23.5).
 constexpr int kFusedSplits = 16;
 constexpr int kMostSequences = 65535; // a launch's z extent
 constexpr size_t kPartialBytes = (size_t) 64 << 20; // a context's room for partial rows
