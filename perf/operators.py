@@ -125,8 +125,7 @@ def _quantise(rows):
     """E4M3 values and exponent bytes of fp32 rows [..., width]: the least power
     of two that brings a row's largest magnitude to 448 or below."""
     mantissa, exponent = torch.frexp(rows.abs().amax(dim=-1))
-    exponent = torch.where(mantissa <= 0.875, exponent - 9, exponent - 8)
-    exponent = torch.where(mantissa == 0, -80, exponent).clamp(-80, 120)
+    exponent = torch.where(mantissa <= 0.875, exponent - 9, exponent - 8).clamp(-80, 120)
     return torch.ldexp(rows, -exponent[..., None]).to(torch.float8_e4m3fn), (exponent + 127).to(torch.uint8)
 
 
