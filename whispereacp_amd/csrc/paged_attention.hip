@@ -783,7 +783,8 @@ __global__ void __launch_bounds__(kJoinWaves* kWave) join_few_kernel(Cache cache
     // sums to zero).
     const int own = min(lane, used - 1);
     const float top = first[own * pitch], sum = lane < used ? first[own * pitch + 1] : 0.f;
-    const float factor = sum == 0.f ? 0.f : __builtin_amdgcn_exp2f(top - wave_max(lane < used ? top : -INFINITY));
+    const float largest = wave_max(lane < used ? top : -INFINITY); // (every lane takes part: not in a branch)
+    const float factor = sum == 0.f ? 0.f : __builtin_amdgcn_exp2f(top - largest);
     const float total = wave_sum(factor * sum);
     const int c0 = min(lane, width - 1), c1 = min(lane + kWave, width - 1);
     float low = 0.f, high = 0.f;
