@@ -11,7 +11,7 @@ import functools
 import numpy as np
 import pytest
 
-from test_gpu_paged import Case, check, ctx, store  # noqa: F401 (ctx: the fixture)
+from test_gpu_paged import Case, attend, check, ctx, store  # noqa: F401 (ctx: the fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +81,16 @@ def test_every_split_counts_once(ctx, given, lifts):  # noqa: F811
 def test_scores_far_below_and_above_zero(ctx, given, floor):  # noqa: F811
     # exp2 of such a score is no fp32 number: only differences of scores may be taken.
     check(ctx, lifted(given, (0.0, 1.0, 0.5), floor))
+
+
+@pytest.mark.parametrize("given", [g for g in CUT_CHUNKS + CUT_ROWS if g[0] in (3, 5, 17, 33)], ids=named)
+def test_a_value_that_is_nan_in_a_faint_split(ctx, given):  # noqa: F811
+    # A weight of 2^-290 times NaN is NaN, as within a split: the rows that see such a
+    # value are not finite in its channel, and finite in the others.
+    case = lifted(given, (-200.0,) + (0.0,) * (given[0] - 1))
+    case.value_rows = case.value_rows.copy()
+    case.value_rows[case.table[0, 0], :, 3, 5] = np.nan
+    case.quantise()
+    got = attend(ctx, case).reshape(case.rows, -1, case.width)[:case.counts[0]]
+    assert np.isnan(got[:, :, 5]).all()
+    assert np.isfinite(np.delete(got, 5, 2)).all()

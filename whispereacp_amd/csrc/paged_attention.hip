@@ -168,6 +168,14 @@ __device__ __forceinline__ float load_shared(const float* at)
     return __hip_atomic_load(const_cast<float*>(at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// What a part of a row (a wave's, a split's) is multiplied by where its parts are put
+// together, the largest of their maxima being `largest`; zero for a part without a key of
+// finite score. Parts count by the product however small it is: NaN times zero is NaN.
+__device__ __forceinline__ float part_factor(float top, float largest)
+{
+    return top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - largest);
+}
+
 // Waves a SIMD the registers are kept to.
 template <int ST, int W, int QT>
 constexpr int kTileOccupancy = QT == 1 && W == 64 && ST != kF32 ? 3 : 2;
@@ -595,12 +603,11 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
             float numerator = 0.f, denominator = 0.f;
 #pragma unroll
             for (int w = 0; w < kWaves; ++w)
-                if (totals[w][at] != 0.f) // (a wave without a key)
-                {
-                    const float factor = __builtin_amdgcn_exp2f(tops[w][at] - largest);
-                    numerator += factor * sums[w][at][c];
-                    denominator += factor * totals[w][at];
-                }
+            {
+                const float factor = part_factor(tops[w][at], largest);
+                numerator += factor * sums[w][at][c];
+                denominator += factor * totals[w][at];
+            }
             if (tl.poisoned)
                 numerator = denominator = __builtin_nanf("");
             if (used == 1)
@@ -654,10 +661,9 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
         float total = 0.f;
         for (int i = lane; i < used; i += kWave)
         {
-            const float part = load_shared(first + i * pitch + 1);
-            const float factor = part == 0.f ? 0.f : __builtin_amdgcn_exp2f(factors[slot * used + i] - largest);
+            const float factor = part_factor(factors[slot * used + i], largest);
             factors[slot * used + i] = factor;
-            total += factor * part; // (a split without a key of finite score sums to zero)
+            total += factor * load_shared(first + i * pitch + 1);
         }
         total = wave_sum(total);
         if (lane == 0)
@@ -679,10 +685,8 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
                 part[w] = load_shared(column + min(w0 + w, used - 1) * pitch);
 #pragma unroll
             for (int w = 0; w < kAtOnce; ++w)
-            {
-                const float factor = w0 + w < used ? factors[slot * used + w0 + w] : 0.f;
-                numerator += factor == 0.f ? 0.f : factor * part[w];
-            }
+                if (w0 + w < used)
+                    numerator += factors[slot * used + w0 + w] * part[w];
         }
         const float denominator = (&totals[0][0])[slot];
         *out_of(tl, query, head, tl.first + slot, width, c) = denominator == 0.f ? 0.f : numerator / denominator;
@@ -736,9 +740,9 @@ __global__ void __launch_bounds__(kJoinWaves* kWave) join_kernel(Cache cache, Ro
         }
 #pragma unroll
         for (int i = 0; i < kJoinAhead; ++i)
-            if (i0 + i * kJoinWaves < used && total[i] != 0.f) // (a split without a key of finite score sums to zero)
+            if (i0 + i * kJoinWaves < used)
             {
-                const float factor = __builtin_amdgcn_exp2f(top[i] - largest);
+                const float factor = part_factor(top[i], largest);
                 low += factor * a[i];
                 high += factor * b[i];
                 denominator += factor * total[i];
@@ -779,12 +783,11 @@ __global__ void __launch_bounds__(kJoinWaves* kWave) join_few_kernel(Cache cache
     const int unit = ((int) blockIdx.z * (int) gridDim.y + (int) blockIdx.y) * cache.heads + head;
     const float* first = partial_row(split, unit, 0, slot, width);
     const size_t pitch = (size_t) split.row_slots * (width + 2);
-    // Lane i holds split i's maximum and sum (a split without a key of finite score
-    // sums to zero).
+    // Lane i holds split i's maximum and sum.
     const int own = min(lane, used - 1);
     const float top = first[own * pitch], sum = lane < used ? first[own * pitch + 1] : 0.f;
     const float largest = wave_max(lane < used ? top : -INFINITY); // (every lane takes part: not in a branch)
-    const float factor = sum == 0.f ? 0.f : __builtin_amdgcn_exp2f(top - largest);
+    const float factor = part_factor(top, largest);
     const float total = wave_sum(factor * sum);
     const int c0 = min(lane, width - 1), c1 = min(lane + kWave, width - 1);
     float low = 0.f, high = 0.f;
@@ -802,9 +805,11 @@ __global__ void __launch_bounds__(kJoinWaves* kWave) join_few_kernel(Cache cache
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i)
         {
-            const float f = i0 + i < used ? __shfl(factor, i0 + i) : 0.f;
-            low += f == 0.f ? 0.f : f * a[i];
-            high += f == 0.f ? 0.f : f * b[i];
+            if (i0 + i >= used)
+                break;
+            const float f = __shfl(factor, i0 + i);
+            low += f * a[i];
+            high += f * b[i];
         }
     }
     float* const out = out_of(tl, query, head, pair, width, 0);
