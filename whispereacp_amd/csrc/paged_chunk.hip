@@ -329,6 +329,7 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FU
 
     // The raw tile to LDS.
     auto stage = [&](int k0, bool apart) {
+        const int page = wave == 0 ? pages[0] : wave == 1 ? pages[1] : wave == 2 ? pages[2] : pages[3]; // of its values
         if (ST == kE4M3 && apart)
         {
             if (key_run == 0)
@@ -341,7 +342,8 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FU
                 {
                     const int key = key_of_value(i), power = (int) value_byte(i) - value_base;
                     value_power[key] = (float) power;
-                    value_inverse[key] = k0 + key < end ? ldexpf(1.f, -power) : 0.f;
+                    // (Of rows that nobody sees, or of no page, it may be anything.)
+                    value_inverse[key] = k0 + key < end && page >= 0 ? ldexpf(1.f, -power) : 0.f;
                 }
         }
 #pragma unroll
@@ -375,7 +377,6 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FU
         // A weight of zero hides a value only while it is finite: values that no pair
         // sees count as zero, and non-finite ones among keys that some pairs see are
         // added behind the products, to those pairs alone.
-        const int page = wave == 0 ? pages[0] : wave == 1 ? pages[1] : wave == 2 ? pages[2] : pages[3];
         if (k0 + kChunkKeys > min(tl.least, end) || page < 0)
         {
             bool odd = false;
