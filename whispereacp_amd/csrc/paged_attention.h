@@ -92,11 +92,11 @@ __device__ __forceinline__ float* partial_row(const Split& split, int unit, int 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32u __attribute__((aligned(1)));
 
-// Two E4M3 bytes (the low or high half of `packed`) as two fp16, exact.
+// Two E4M3 bytes (the low or high half of `packed`) times a power of two as two fp16.
 template <bool HIGH>
-__device__ __forceinline__ uint32_t e4m3_to_halves(uint32_t packed)
+__device__ __forceinline__ uint32_t e4m3_to_halves(uint32_t packed, float power)
 {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) packed, 1.f, HIGH));
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) packed, power, HIGH));
 }
 
 // What the matrix cores multiply a storage as, and its bytes.
@@ -149,6 +149,50 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t pair)
     if ((pair & (kTop << 16)) != kTop << 16)
         kept |= pair & 0xFFFF0000u;
     return kept;
+}
+
+// E4M3 values as operands. A row's values times its power of two, relative to a base,
+// are fp16 values exactly where the power is 2^kLeastShift to 2^kMostShift of the base's.
+// A tile of keys with another power among them (a row of zeros has the least there is)
+// goes as bf16, which holds four significant bits at any power, and its weights in three
+// bf16 parts, exact: a quarter more products, and no power or weight is out of reach.
+// What is summed leaves out the base: the first key's power within kLeastBase and
+// kMostBase; from the first such tile on kLeastBase, near which ordinary rows lie; from
+// one with a power past kLoudest on kLoudBase, where neither fp32's largest values pass
+// its range as sums nor the least rows bf16's. (All as exponent bytes.)
+constexpr int kLeastShift = -15, kMostShift = 7;
+constexpr int kLeastBase = kExponentBias - 7, kMostBase = kExponentBias + 34;
+constexpr int kLoudest = kExponentBias + 64, kLoudBase = kExponentBias + 35;
+
+// Rows and sums of E4M3 values leave a kernel's loop times 2^-kSumShift: without the
+// weights' bias of 2^14, and so that the values nearest fp32's end can be summed.
+constexpr int kSumShift = 34;
+
+__device__ __forceinline__ int first_base(int byte)
+{
+    return min(max(byte, kLeastBase), kMostBase);
+}
+
+// The base of a tile whose powers `base` does not take.
+__device__ __forceinline__ int wide_base(int base, bool loud)
+{
+    return base == kLoudBase || loud ? kLoudBase : kLeastBase;
+}
+
+// Whether powers from `low` to `high` fit the operands.
+__device__ __forceinline__ bool base_takes(int base, int low, int high)
+{
+    return low - base >= kLeastShift && high - base <= kMostShift;
+}
+
+// Two E4M3 bytes (the low or high half of `packed`) times 2^shift as two bf16, exact
+// (magnitudes past fp32's range become infinities).
+template <bool HIGH>
+__device__ __forceinline__ uint32_t e4m3_to_bf16(uint32_t packed, int shift)
+{
+    const auto pair = __builtin_amdgcn_cvt_pk_f32_fp8((int) packed, HIGH);
+    return __builtin_amdgcn_perm(__float_as_uint(ldexpf(pair[1], shift)), __float_as_uint(ldexpf(pair[0], shift)),
+                                 0x07060302);
 }
 
 // A stored value widened, E4M3 without its row's power.

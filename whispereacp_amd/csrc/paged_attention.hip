@@ -47,10 +47,9 @@ __device__ __forceinline__ float groups_sum(float v)
 // q, and the weights, go in 16-bit parts (cut_pair), so a product with what the
 // storage holds is as exact as fp32's; fp16 parts of q are of q·2^-e, e from the
 // pair's largest magnitude, and the weights are exp2(s - max + 14), which puts
-// both far from fp16's ends. An E4M3 value row's power of two 2^v would take a
-// weight past them, so the maximum is that of s + v and the parts those of
-// exp2(s + v - max + 14); the sum takes the weights times 2^-v. fp32 storage runs
-// in fp32.
+// both far from fp16's ends. An E4M3 key row's power of two multiplies its scores, a
+// value row's its operands (relative to a base: paged_attention.h), so weights, maxima
+// and sums are those of the scores alone. fp32 storage runs in fp32.
 //
 // Bound by the cache's read where rows are few and sequences long: a wave keeps the
 // next 32 keys and values in flight while it works on these. One token over 131072
@@ -108,6 +107,11 @@ __device__ __forceinline__ void load_tile(const Cache& cache, const Pages& pages
         const int page = second ? pages.page[1] : pages.page[0];
         t.bad[b] = page < 0;
         const size_t row = pool_row(max(page, 0), head, (second ? k0 + 16 : k0) & mask, cache.heads, cache.page_shift);
+        if constexpr (ST == kE4M3) // (looked at first)
+        {
+            t.ke[b] = *(const __attribute__((address_space(1))) u32u*) (cache.key_exponents + row + (uint32_t) (4 * g));
+            t.ve[b] = *(const __attribute__((address_space(1))) u32u*) (cache.value_exponents + row + (uint32_t) (4 * g));
+        }
         const char* keys = static_cast<const char*>(cache.keys) + row * row_bytes;
         const char* values = static_cast<const char*>(cache.values) + row * row_bytes;
         constexpr int kRuns = W * bytes_of<ST> / 64;
@@ -124,11 +128,6 @@ __device__ __forceinline__ void load_tile(const Cache& cache, const Pages& pages
 #pragma unroll
         for (int r = 0; r < 4; ++r)
             load_words(values + r * row_bytes + at.value, t.v[b][r]);
-        if constexpr (ST == kE4M3)
-        {
-            t.ke[b] = *(const __attribute__((address_space(1))) u32u*) (cache.key_exponents + row + (uint32_t) (4 * g));
-            t.ve[b] = *(const __attribute__((address_space(1))) u32u*) (cache.value_exponents + row + (uint32_t) (4 * g));
-        }
     }
 }
 
@@ -139,19 +138,35 @@ __device__ __forceinline__ u32x4 key_operand(const Tile<ST, W>& t, int b, int j)
     if constexpr (ST == kE4M3)
     {
         const uint32_t x = t.k[b][2 * j], y = t.k[b][2 * j + 1];
-        return u32x4 {e4m3_to_halves<false>(x), e4m3_to_halves<true>(x), e4m3_to_halves<false>(y),
-                      e4m3_to_halves<true>(y)};
+        return u32x4 {e4m3_to_halves<false>(x, 1.f), e4m3_to_halves<true>(x, 1.f), e4m3_to_halves<false>(y, 1.f),
+                      e4m3_to_halves<true>(y, 1.f)};
     }
     else
         return u32x4 {t.k[b][4 * j], t.k[b][4 * j + 1], t.k[b][4 * j + 2], t.k[b][4 * j + 3]};
 }
 
-// Channels 2i and 2i + 1 of a stored value row, 16 bits each.
-template <int ST, int W>
-__device__ __forceinline__ uint32_t value_pair(const Tile<ST, W>& t, int b, int r, int i)
+// The exponent byte of the key (value) row 16b + 4g + r.
+__device__ __forceinline__ int exponent_of(const uint32_t (&rows)[2], int b, int r)
 {
-    if constexpr (ST == kE4M3)
-        return i % 2 == 0 ? e4m3_to_halves<false>(t.v[b][r][i / 2]) : e4m3_to_halves<true>(t.v[b][r][i / 2]);
+    return (int) (rows[b] >> (8 * r) & 255u);
+}
+
+// Channels 2i and 2i + 1 of a stored value row, 16 bits each of type VT; E4M3 ones
+// times their row's power relative to the base.
+template <int ST, int VT, int W>
+__device__ __forceinline__ uint32_t value_pair(const Tile<ST, W>& t, int b, int r, int i, int base)
+{
+    if constexpr (ST == kE4M3 && VT == kBF16)
+    {
+        const int shift = exponent_of(t.ve, b, r) - base;
+        return i % 2 == 0 ? e4m3_to_bf16<false>(t.v[b][r][i / 2], shift) : e4m3_to_bf16<true>(t.v[b][r][i / 2], shift);
+    }
+    else if constexpr (ST == kE4M3)
+    {
+        const float power = __uint_as_float((uint32_t) (exponent_of(t.ve, b, r) + kExponentBias - base) << 23);
+        return i % 2 == 0 ? e4m3_to_halves<false>(t.v[b][r][i / 2], power)
+                          : e4m3_to_halves<true>(t.v[b][r][i / 2], power);
+    }
     else
         return t.v[b][r][i];
 }
@@ -166,6 +181,134 @@ __device__ __forceinline__ void store_shared(float* at, float value)
 __device__ __forceinline__ float load_shared(const float* at)
 {
     return __hip_atomic_load(const_cast<float*>(at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// The weights of 32 keys (4g + r of either sixteen) for 16·QT pairs, in parts for values
+// of type VT.
+template <int VT_, int QT>
+struct Weights
+{
+    static constexpr int VT = VT_;
+    uint32_t part[QT][parts_of<VT>()][VT == kF32 ? 8 : 4];
+};
+
+// Pair t's from its scores; their sum joins l.
+template <int VT, int QT>
+__device__ __forceinline__ void weigh(float4v (&s)[2], float offset, int t, Weights<VT, QT>& weights, float& l)
+{
+    float own = 0.f;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+        {
+            s[b][r] = __builtin_amdgcn_exp2f(s[b][r] - offset);
+            own += s[b][r];
+        }
+    l += own;
+#pragma unroll
+    for (int i = 0; i < (VT == kF32 ? 8 : 4); ++i)
+        if constexpr (VT == kF32)
+            weights.part[t][0][i] = __float_as_uint(s[i / 4][i % 4]);
+        else
+        {
+            uint32_t cut[3];
+            cut_pair<VT>(s[i / 2][2 * (i % 2)], s[i / 2][2 * (i % 2) + 1], cut);
+#pragma unroll
+            for (int p = 0; p < parts_of<VT>(); ++p)
+                weights.part[t][p][i] = cut[p];
+        }
+}
+
+// Adds 32 keys' value rows, as type VT, by their weights to the pairs' rows, two channels
+// of each lane's at a time. A weight of zero hides a value only while it is finite: the
+// careful way counts values that no pair sees (`shown`) as zero, and where some pairs see
+// a key and others do not (`mixed`), non-finite values too; `odd` tells of those.
+template <int ST, int VT, int W, int QT>
+__device__ __forceinline__ void add_rows(const Tile<ST, W>& kv, int base, const Weights<VT, QT>& weights, bool careful,
+                                         bool mixed, const uint32_t (&shown)[4], float4v (&o)[QT][W / 16], bool& odd)
+{
+    constexpr int CPL = W / 16;
+#pragma unroll
+    for (int c = 0; c < CPL; c += 2)
+    {
+        // Channels CPL·li + c and + c + 1 of keys 16b + 4g + r.
+        if constexpr (VT == kF32)
+        {
+            float v[2][8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    v[e][i] = __uint_as_float(kv.v[i / 4][i % 4][c + e]);
+            if (careful)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        if ((shown[i / 2] & (i % 2 == 0 ? 0xFFFFu : 0xFFFF0000u)) == 0)
+                            v[e][i] = 0.f;
+            if (mixed)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                    {
+                        odd = odd || !isfinite(v[e][i]);
+                        v[e][i] = isfinite(v[e][i]) ? v[e][i] : 0.f;
+                    }
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        o[t][c + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                            v[e][i], __uint_as_float(weights.part[t][0][i]), o[t][c + e], 0, 0, 0);
+                }
+        }
+        else
+        {
+            u32x4 v[2];
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+            {
+                const uint32_t x = value_pair<ST, VT>(kv, d / 2, 2 * (d % 2), c / 2, base);
+                const uint32_t y = value_pair<ST, VT>(kv, d / 2, 2 * (d % 2) + 1, c / 2, base);
+                v[0][d] = __builtin_amdgcn_perm(y, x, 0x05040100); // the low halves
+                v[1][d] = __builtin_amdgcn_perm(y, x, 0x07060302); // the high ones
+            }
+            if (careful)
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        v[e][d] &= shown[d];
+            if (mixed)
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                    {
+                        const uint32_t kept = finite_halves<VT>(v[e][d]);
+                        odd = odd || kept != v[e][d];
+                        v[e][d] = kept;
+                    }
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                {
+#pragma unroll
+                    for (int p = parts_of<VT>() - 1; p >= 0; --p)
+                        o[t][c + e] = mfma16<VT>(v[e],
+                                                 u32x4 {weights.part[t][p][0], weights.part[t][p][1],
+                                                        weights.part[t][p][2], weights.part[t][p][3]},
+                                                 o[t][c + e]);
+                }
+        }
+    }
 }
 
 // What a part of a row (a wave's, a split's) is multiplied by where its parts are put
@@ -224,7 +367,8 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
 
     // The queries: lane (li, g) holds the channels of pair li that it holds of a key.
     uint32_t qp[QT][OT == kF32 ? 1 : kParts][OT == kF32 ? W / 4 : W / 8];
-    float left[QT]; // the power of two that the parts leave out
+    float left[QT]; // the power of two that the parts leave out,
+    int lift[QT];   // E4M3: its exponent less a key byte's bias
     int seen[QT];
 #pragma unroll
     for (int t = 0; t < QT; ++t)
@@ -248,6 +392,7 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
                 x[i + j] = run[j] * query.scale;
         }
         left[t] = 1.f;
+        lift[t] = 0;
         if constexpr (OT == kF32)
 #pragma unroll
             for (int i = 0; i < W / 4; ++i)
@@ -268,6 +413,7 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
                 for (int i = 0; i < W / 4; ++i)
                     x[i] = ldexpf(x[i], shift);
                 left[t] = ldexpf(1.f, -shift);
+                lift[t] = -shift - kExponentBias;
             }
 #pragma unroll
             for (int i = 0; i < W / 8; ++i)
@@ -293,14 +439,58 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
             o[t][c] = float4v {0.f, 0.f, 0.f, 0.f};
     }
 
+    int base = kExponentBias; // E4M3: the power that the value operands leave out
+    if (ST == kE4M3 && k0 < end)
+        base = first_base((int) (__builtin_amdgcn_readfirstlane(now.ve[0]) & 255u));
+
     auto work = [&](const Tile<ST, W>& kv, int k0) {
         // Keys that not every pair sees, or whose page is none, take the careful way.
         const bool careful = k0 + kKeys > min(tl.least, end) || kv.bad[0] || kv.bad[1];
-        uint32_t weights[QT][OT == kF32 ? 1 : kParts][OT == kF32 ? 8 : 4];
+        bool wide = false; // E4M3: the values go as bf16
+        if constexpr (ST == kE4M3)
+        {
+            int low = 255, high = 0;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                {
+                    low = min(low, exponent_of(kv.ve, b, r));
+                    high = max(high, exponent_of(kv.ve, b, r));
+                }
+            if (careful) // (rows that nobody sees may hold anything)
+            {
+                low = high = base;
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (!kv.bad[b] && k0 + 16 * b + 4 * g + r < end)
+                        {
+                            low = min(low, exponent_of(kv.ve, b, r));
+                            high = max(high, exponent_of(kv.ve, b, r));
+                        }
+            }
+            if (__any(!base_takes(base, low, high))) // (rare)
+            {
+                const int next = wide_base(base, __any(high > kLoudest));
+                const float by = ldexpf(1.f, base - next);
+#pragma unroll
+                for (int t = 0; t < QT; ++t)
+#pragma unroll
+                    for (int c = 0; c < CPL; ++c)
+                        o[t][c] *= by;
+                base = next;
+                wide = __any(!base_takes(base, low, high));
+            }
+        }
+        float offset[QT];      // from scores to the weights' powers
+        float4v scores[QT][2]; // of keys 4g + r of either sixteen
+        Weights<OT, QT> weights;
 #pragma unroll
         for (int t = 0; t < QT; ++t)
         {
-            float4v s[2];
+            float4v (&s)[2] = scores[t];
 #pragma unroll
             for (int b = 0; b < 2; ++b)
             {
@@ -333,23 +523,15 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
                     }
                 }
             }
-            // Scores in powers of two; E4M3 ones with the value rows' powers in them.
-            float inverse[2][4];
+            // Scores in powers of two.
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                {
                     if constexpr (ST == kE4M3)
-                    {
-                        const uint32_t ke = kv.ke[b] >> (8 * r) & 255u, ve = kv.ve[b] >> (8 * r) & 255u;
-                        s[b][r] = __builtin_fmaf(s[b][r], left[t] * __uint_as_float(ke << 23),
-                                                 (float) ve - (float) kExponentBias);
-                        inverse[b][r] = __uint_as_float((254u - ve) << 23);
-                    }
+                        s[b][r] = ldexpf(s[b][r], exponent_of(kv.ke, b, r) + lift[t]);
                     else if constexpr (OT == kF16)
                         s[b][r] *= left[t];
-                }
             if (careful)
             {
 #pragma unroll
@@ -359,8 +541,6 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
                     {
                         if (kv.bad[b])
                             s[b][r] = __builtin_nanf("");
-                        if (ST == kE4M3 && (kv.bad[b] || k0 + 16 * b + 4 * g + r >= end))
-                            inverse[b][r] = 0.f;
                         s[b][r] = k0 + 16 * b + 4 * g + r < seen[t] ? s[b][r] : -INFINITY;
                     }
             }
@@ -374,7 +554,8 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
             // and the bias stay exact however often it grows. (Before a key of finite
             // score, zero in its place: the weights are zero.)
             const float m_new = fmaxf(m[t], ceilf(groups_max(top)));
-            const float finite = m_new == -INFINITY ? 0.f : m_new, base = finite - kBias;
+            const float finite = m_new == -INFINITY ? 0.f : m_new;
+            offset[t] = finite - kBias;
             if (__any(m_new != m[t])) // (seldom, but for the first keys)
             {
                 const float alpha = __builtin_amdgcn_exp2f(m[t] - finite);
@@ -384,33 +565,11 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
                     o[t][c] *= alpha;
                 m[t] = m_new;
             }
-            float own = 0.f;
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                {
-                    s[b][r] = __builtin_amdgcn_exp2f(s[b][r] - base);
-                    own += ST == kE4M3 ? s[b][r] * inverse[b][r] : s[b][r];
-                }
-            l[t] += own;
-#pragma unroll
-            for (int i = 0; i < (OT == kF32 ? 8 : 4); ++i)
-                if constexpr (OT == kF32)
-                    weights[t][0][i] = __float_as_uint(s[i / 4][i % 4]);
-                else
-                {
-                    uint32_t cut[3];
-                    cut_pair<OT>(s[i / 2][2 * (i % 2)], s[i / 2][2 * (i % 2) + 1], cut);
-#pragma unroll
-                    for (int p = 0; p < kParts; ++p)
-                        weights[t][p][i] = cut[p];
-                }
+            if constexpr (ST != kE4M3)
+                weigh(scores[t], offset[t], t, weights, l[t]);
         }
 
-        // The rows, two channels of each lane's at a time. A weight of zero hides a value
-        // only while it is finite: the careful way counts values that no pair sees as
-        // zero, and where some pairs see a key and others do not, non-finite values are
+        // The rows. Non-finite values of keys that some pairs see and others do not are
         // added behind the products, to those that see them alone.
         bool odd = false;
         const bool mixed = careful && tl.least < tl.most;
@@ -422,85 +581,21 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
                 const int key = k0 + 16 * (d / 2) + 4 * g + 2 * (d % 2);
                 shown[d] = kv.bad[d / 2] ? 0u : (key < end ? 0xFFFFu : 0u) | (key + 1 < end ? 0xFFFF0000u : 0u);
             }
-#pragma unroll
-        for (int c = 0; c < CPL; c += 2)
+        if (ST == kE4M3 && wide)
         {
-            // Channels CPL·li + c and + c + 1 of keys 16b + 4g + r.
-            if constexpr (OT == kF32)
-            {
-                float v[2][8];
+            Weights<kBF16, QT> parts;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        v[e][i] = __uint_as_float(kv.v[i / 4][i % 4][c + e]);
-                if (careful)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            if ((shown[i / 2] & (i % 2 == 0 ? 0xFFFFu : 0xFFFF0000u)) == 0)
-                                v[e][i] = 0.f;
-                if (mixed)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                        {
-                            odd = odd || !isfinite(v[e][i]);
-                            v[e][i] = isfinite(v[e][i]) ? v[e][i] : 0.f;
-                        }
+            for (int t = 0; t < QT; ++t)
+                weigh(scores[t], offset[t], t, parts, l[t]);
+            add_rows(kv, base, parts, careful, mixed, shown, o, odd);
+        }
+        else
+        {
+            if constexpr (ST == kE4M3)
 #pragma unroll
                 for (int t = 0; t < QT; ++t)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                    {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            o[t][c + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                v[e][i], __uint_as_float(weights[t][0][i]), o[t][c + e], 0, 0, 0);
-                    }
-            }
-            else
-            {
-                u32x4 v[2];
-#pragma unroll
-                for (int d = 0; d < 4; ++d)
-                {
-                    const uint32_t x = value_pair<ST, W>(kv, d / 2, 2 * (d % 2), c / 2);
-                    const uint32_t y = value_pair<ST, W>(kv, d / 2, 2 * (d % 2) + 1, c / 2);
-                    v[0][d] = __builtin_amdgcn_perm(y, x, 0x05040100); // the low halves
-                    v[1][d] = __builtin_amdgcn_perm(y, x, 0x07060302); // the high ones
-                }
-                if (careful)
-#pragma unroll
-                    for (int d = 0; d < 4; ++d)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            v[e][d] &= shown[d];
-                if (mixed)
-#pragma unroll
-                    for (int d = 0; d < 4; ++d)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                        {
-                            const uint32_t kept = finite_halves<OT>(v[e][d]);
-                            odd = odd || kept != v[e][d];
-                            v[e][d] = kept;
-                        }
-#pragma unroll
-                for (int t = 0; t < QT; ++t)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                    {
-#pragma unroll
-                        for (int p = kParts - 1; p >= 0; --p)
-                            o[t][c + e] = mfma16<OT>(v[e],
-                                                     u32x4 {weights[t][p][0], weights[t][p][1], weights[t][p][2],
-                                                            weights[t][p][3]},
-                                                     o[t][c + e]);
-                    }
-            }
+                    weigh(scores[t], offset[t], t, weights, l[t]);
+            add_rows(kv, base, weights, careful, mixed, shown, o, odd);
         }
         if (mixed && __any(odd)) // (rare: infinities or NaN among the new rows' values)
 #pragma unroll
@@ -508,25 +603,31 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
             {
                 constexpr int kDwords = OT == kF32 ? 8 : 4;
                 uint32_t parts[kDwords]; // (opaque: nothing of this is worked out before it is needed)
+                if constexpr (ST != kE4M3)
 #pragma unroll
-                for (int i = 0; i < kDwords; ++i)
-                {
-                    parts[i] = weights[t][0][i];
-                    asm("" : "+v"(parts[i]));
-                }
+                    for (int i = 0; i < kDwords; ++i)
+                    {
+                        parts[i] = weights.part[t][0][i];
+                        asm("" : "+v"(parts[i]));
+                    }
 #pragma unroll 1
                 for (int key = 0; key < kKeys; ++key)
                 {
-                    // Key 16b + 4g + r is held by lane group g. (Only that its weight is
-                    // not zero matters: the first part of it does.)
-                    uint32_t held = 0;
+                    // Key 16b + 4g + r is held by lane group g. (Only that its weight is not zero
+                    // matters: the first part of it does. E4M3 has no infinities, and NaN is NaN
+                    // by any weight.)
+                    float weight = 1.f;
+                    if constexpr (ST != kE4M3)
+                    {
+                        uint32_t held = 0;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (4 * (key / 16) + key % 4 == i)
-                            held = OT == kF32   ? parts[i * kDwords / 8]
-                                   : i % 2 == 0 ? parts[i * kDwords / 8] << 16
-                                                : parts[i * kDwords / 8] & 0xFFFF0000u;
-                    const float weight = __uint_as_float(__shfl(held, li + 16 * (key / 4 % 4)));
+                        for (int i = 0; i < 8; ++i)
+                            if (4 * (key / 16) + key % 4 == i)
+                                held = OT == kF32   ? parts[i * kDwords / 8]
+                                       : i % 2 == 0 ? parts[i * kDwords / 8] << 16
+                                                    : parts[i * kDwords / 8] & 0xFFFF0000u;
+                        weight = __uint_as_float(__shfl(held, li + 16 * (key / 4 % 4)));
+                    }
                     const int position = k0 + key;
                     const int page = page_of(table, rows.table_width, cache.page_shift, cache.pages, position);
                     if (position >= seen[t] || page < 0)
@@ -575,7 +676,8 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
 #pragma unroll
     for (int t = 0; t < QT; ++t)
     {
-        const float total = groups_sum(l[t]);
+        const float total = groups_sum(l[t]) * (ST == kE4M3 ? ldexpf(1.f, -kSumShift) : 1.f);
+        const float power = ST == kE4M3 ? ldexpf(1.f, base - kExponentBias - kSumShift) : 1.f;
         if (t > 0)
             __syncthreads(); // (the rows before are read)
         if (g == 0)
@@ -589,7 +691,7 @@ __global__ void __launch_bounds__(kTileWaves* kWave, (kTileOccupancy<ST, W, QT>)
 #pragma unroll
                 for (int c = 0; c < CPL; c += 4)
                     *reinterpret_cast<float4v*>(&sums[wave][li][CPL * (4 * g + r) + c]) =
-                        float4v {o[t][c][r], o[t][c + 1][r], o[t][c + 2][r], o[t][c + 3][r]};
+                        float4v {o[t][c][r], o[t][c + 1][r], o[t][c + 2][r], o[t][c + 3][r]} * power;
         __syncthreads();
         for (int i = threadIdx.x; i < 16 * W; i += kWaves * kWave)
         {

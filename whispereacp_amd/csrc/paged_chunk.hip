@@ -55,10 +55,10 @@ __device__ __forceinline__ void lds_barrier()
 // the weights cross no lanes.
 //
 // Queries and weights go in 16-bit parts, with the scalings of the kernel for few
-// rows. E4M3 rows' powers of two are multiplied into the 16-bit operands,
-// relative to the first key's: an E4M3 value times 2^-15 .. 2^7 is an fp16 value
-// exactly. A tile with a power outside that keeps its rows as they are and takes the
-// few rows' way: powers of keys multiply the scores, powers of values join them.
+// rows. E4M3 rows' powers of two are multiplied into the 16-bit operands, relative to a
+// base (paged_attention.h; the keys' is their first one's). A tile with a key's power
+// outside what they take keeps its keys as they are and multiplies their scores; one
+// with such a value row goes as bf16 for the value products.
 //
 // While a tile is worked on the next is in flight to registers, and two blocks a CU
 // fill each other's barriers; a wave at the matrix cores goes before one at vector
@@ -72,8 +72,6 @@ __device__ __forceinline__ void lds_barrier()
 // keys are summed apart, at 32 more vector instructions a tile.
 // ---------------------------------------------------------------------------
 constexpr int kChunkWaves = 4, kChunkKeys = 64;
-constexpr int kLeastShift = -15, kMostShift = 7;
-constexpr int kLeastBase = -7, kMostBase = 46; // rows' powers are 2^-80 to 2^120
 
 // The 16-byte run of run c of eight keys of a channel's row: eight consecutive
 // rows, and every fourth of 32, lie in different bank groups.
@@ -91,17 +89,16 @@ __device__ __forceinline__ int key_slot(int key, int c)
 // Eight E4M3 bytes times 2^power (as a float) as fp16.
 __device__ __forceinline__ u32x4 e4m3_run(uint32_t low, uint32_t high, float power)
 {
-    auto pair = [&](uint32_t packed, auto top) {
-        return __builtin_bit_cast(uint32_t,
-                                  __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) packed, power, decltype(top)::value));
-    };
-    return u32x4 {pair(low, std::false_type {}), pair(low, std::true_type {}), pair(high, std::false_type {}),
-                  pair(high, std::true_type {})};
+    return u32x4 {e4m3_to_halves<false>(low, power), e4m3_to_halves<true>(low, power),
+                  e4m3_to_halves<false>(high, power), e4m3_to_halves<true>(high, power)};
 }
 
-// Waves a SIMD: two, or one where the registers of two would spill into the loop.
+// Waves a SIMD: three (E4M3 heads of 64, 512 rows over 2048 keys of 12 heads, 16 sequences:
+// 219 us with two), two, or one, as many as do not make the registers spill into the loop.
 template <int ST, int C, bool FULL>
-constexpr int kChunkOccupancy = (ST == kBF16 && C >= 96) || (!FULL && C == 128) ? 1 : 2;
+constexpr int kChunkOccupancy = (ST == kBF16 && C >= 96) || (!FULL && C == 128) ? 1
+                                : ST != kBF16 && FULL && C == 64                ? 3
+                                                                                : 2;
 
 // Heads lie in LDS as W channels (64 or 128), of which C are worked on (a multiple of
 // 32); FULL: the heads are C wide.
@@ -118,10 +115,11 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FU
     constexpr int kValueWords = (kValueChannels * bytes_of<ST> + 3) / 4;
     __shared__ u32x4 ks[kChunkKeys * W / 8];
     __shared__ u32x4 vs[W * kChunkKeys / 8];
-    __shared__ __align__(16) float key_power[kChunkKeys], value_power[kChunkKeys], value_inverse[kChunkKeys];
-    // The last tile (its first key + 1) with a non-finite value that some pair sees,
-    // and the last E4M3 one whose rows' powers are not in the operands.
-    __shared__ int odd_tile, apart_tile;
+    __shared__ __align__(16) int key_power[kChunkKeys];
+    // The last tile (its first key + 1) with a non-finite value that some pair sees, and
+    // the last E4M3 ones whose keys' and values' powers the operands do not take, and
+    // with a value's past kLoudest.
+    __shared__ int odd_tile, apart_tile, wide_tile, loud_tile;
 
     const int which = blockIdx.x % split.splits, head = blockIdx.x / split.splits;
     const int sequence = first_sequence + blockIdx.z;
@@ -146,7 +144,7 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FU
     const int wave_least = first <= tl.last ? min(keys_seen(query, tl, first), end) : 0;
     const int wave_most = first <= tl.last ? min(keys_seen(query, tl, min(first + 31, tl.last)), end) : 0;
     u32x4 qp[C / 16][kParts];
-    float unit = 1.f; // the power of two that the parts leave out
+    int shift = 0; // the parts are the query's times 2^shift
     {
         const float* at = query.q + (size_t) (tl.first_row + (real ? pair : tl.first) / query.group) * query.q_stride
                           + (size_t) (head * query.group + (real ? pair : tl.first) % query.group) * width;
@@ -167,13 +165,11 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FU
                     top = fmaxf(top, fabsf(x[j][i + e]));
                 }
             }
-        int shift = 0;
         if constexpr (OT == kF16)
         {
             // 2^13 <= top·2^shift < 2^14 (a pair of zeros, or not finite: as it is)
             top = halves_max(top);
             shift = top > 0.f && top < INFINITY ? min(140 - (int) (__float_as_uint(top) >> 23), 126) : 0;
-            unit = ldexpf(1.f, -shift);
         }
 #pragma unroll
         for (int j = 0; j < C / 16; ++j)
@@ -252,20 +248,16 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FU
                                                                              + (uint32_t) (4 * h));
     };
 
-    // E4M3: the powers that the operands leave out, those of the first key's rows, or
-    // the nearest that keep every other row's within a float's range of them.
+    // E4M3: the powers that the operands leave out.
     int key_base = kExponentBias, value_base = kExponentBias;
     if (ST == kE4M3 && begin < end)
     {
         const int page = page_of(table, rows.table_width, cache.page_shift, cache.pages, begin);
         const size_t row = pool_row(max(page, 0), head, begin & page_mask, cache.heads, cache.page_shift);
-        auto base_of = [&](const uint8_t* exponents) {
-            return min(max((int) exponents[row], kExponentBias + kLeastBase), kExponentBias + kMostBase);
-        };
-        key_base = base_of(cache.key_exponents);
-        value_base = base_of(cache.value_exponents);
+        key_base = first_base(cache.key_exponents[row]);
+        value_base = first_base(cache.value_exponents[row]);
     }
-    // 2^(byte - base) as a float's bits, for bytes within a float's range of the base.
+    // 2^(byte - base) as a float's bits, for bytes that a base takes.
     auto power_bits = [](uint32_t byte, int base) { return (byte + (uint32_t) (kExponentBias - base)) << 23; };
     auto value_byte = [&](int i) { return raw.ve[i / 4] >> (8 * (i % 4)) & 255u; };
     auto key_of_value = [&](int i) { return 16 * wave + 8 * (i / 4) + 4 * h + i % 4; };
@@ -278,8 +270,7 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FU
         return bad;
     };
 
-    // Before the barrier behind which the tile goes to LDS: whether its rows' powers
-    // do not all fit the operands.
+    // Before the barrier behind which the tile goes to LDS: what its rows' powers ask for.
     auto look = [&](int k0) {
         if constexpr (ST == kE4M3)
         {
@@ -313,7 +304,8 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FU
                 low = min(low, key_bytes[i]);
                 high = max(high, key_bytes[i]);
             }
-            bool fits = low - key_base >= kLeastShift && high - key_base <= kMostShift;
+            if (!base_takes(key_base, low, high))
+                apart_tile = k0 + 1;
             low = high = value_bytes[0];
 #pragma unroll
             for (int i = 1; i < 8; ++i)
@@ -321,31 +313,22 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FU
                 low = min(low, value_bytes[i]);
                 high = max(high, value_bytes[i]);
             }
-            fits = fits && low - value_base >= kLeastShift && high - value_base <= kMostShift;
-            if (!fits)
-                apart_tile = k0 + 1;
+            if (!base_takes(value_base, low, high))
+            {
+                wide_tile = k0 + 1;
+                if (high > kLoudest)
+                    loud_tile = k0 + 1;
+            }
         }
     };
 
     // The raw tile to LDS.
-    auto stage = [&](int k0, bool apart) {
-        const int page = wave == 0 ? pages[0] : wave == 1 ? pages[1] : wave == 2 ? pages[2] : pages[3]; // of its values
-        if (ST == kE4M3 && apart)
-        {
-            if (key_run == 0)
+    auto stage = [&](int k0, bool apart, auto type) __attribute__((always_inline)) {
+        constexpr int VT = decltype(type)::value;
+        if (ST == kE4M3 && apart && key_run == 0)
 #pragma unroll
-                for (int i = 0; i < kKeyRuns; ++i)
-                    key_power[key_of + kKeysAtOnce * i] = ldexpf(1.f, (int) raw.ke[i] - key_base);
-            if (threadIdx.x % 32 == 0)
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                {
-                    const int key = key_of_value(i), power = (int) value_byte(i) - value_base;
-                    value_power[key] = (float) power;
-                    // (Of rows that nobody sees, or of no page, it may be anything.)
-                    value_inverse[key] = k0 + key < end && page >= 0 ? ldexpf(1.f, -power) : 0.f;
-                }
-        }
+            for (int i = 0; i < kKeyRuns; ++i)
+                key_power[key_of + kKeysAtOnce * i] = (int) raw.ke[i] - kExponentBias;
 #pragma unroll
         for (int i = 0; i < kKeyRuns; ++i)
         {
@@ -363,20 +346,28 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FU
         uint32_t pairs[8][kValueChannels / 2];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-        {
-            const float power = ST == kE4M3 && !apart ? __uint_as_float(power_bits(value_byte(i), value_base)) : 1.f;
+            if constexpr (ST == kE4M3 && VT == kBF16)
+            {
+                const int power = (int) value_byte(i) - value_base;
+                pairs[i][0] = e4m3_to_bf16<false>(raw.v[i][0], power);
+                if constexpr (kValueChannels > 2)
+                    pairs[i][1] = e4m3_to_bf16<true>(raw.v[i][0], power);
+            }
+            else if constexpr (ST == kE4M3)
+            {
+                const float power = __uint_as_float(power_bits(value_byte(i), value_base));
+                pairs[i][0] = e4m3_to_halves<false>(raw.v[i][0], power);
+                if constexpr (kValueChannels > 2)
+                    pairs[i][1] = e4m3_to_halves<true>(raw.v[i][0], power);
+            }
+            else
 #pragma unroll
-            for (int c = 0; c < kValueChannels / 2; ++c)
-                if constexpr (ST == kE4M3)
-                    pairs[i][c] = __builtin_bit_cast(
-                        uint32_t, c == 0 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) raw.v[i][0], power, false)
-                                         : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int) raw.v[i][0], power, true));
-                else
+                for (int c = 0; c < kValueChannels / 2; ++c)
                     pairs[i][c] = raw.v[i][c];
-        }
         // A weight of zero hides a value only while it is finite: values that no pair
         // sees count as zero, and non-finite ones among keys that some pairs see are
         // added behind the products, to those pairs alone.
+        const int page = wave == 0 ? pages[0] : wave == 1 ? pages[1] : wave == 2 ? pages[2] : pages[3];
         if (k0 + kChunkKeys > min(tl.least, end) || page < 0)
         {
             bool odd = false;
@@ -387,7 +378,7 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FU
 #pragma unroll
                 for (int c = 0; c < kValueChannels / 2; ++c)
                 {
-                    const uint32_t kept = unseen ? 0u : finite_halves<OT>(pairs[i][c]);
+                    const uint32_t kept = unseen ? 0u : finite_halves<VT>(pairs[i][c]);
                     odd = odd || (!unseen && kept != pairs[i][c]);
                     pairs[i][c] = kept;
                 }
@@ -416,7 +407,7 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FU
         o[c] = float16v {};
     float m = -INFINITY, l = 0.f;
     if (threadIdx.x == 0)
-        odd_tile = apart_tile = 0;
+        odd_tile = apart_tile = wide_tile = loud_tile = 0;
     __syncthreads();
 
     if (begin < end)
@@ -425,10 +416,22 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FU
     {
         look(k0);
         lds_barrier(); // (the tile before is read)
-        const bool apart = ST == kE4M3 && apart_tile == k0 + 1;
-        stage(k0, apart);
+        const bool apart = ST == kE4M3 && apart_tile == k0 + 1, wide = ST == kE4M3 && wide_tile == k0 + 1;
+        if (ST == kE4M3 && wide)
+        {
+            const int next = wide_base(value_base, loud_tile == k0 + 1);
+            const float by = ldexpf(1.f, value_base - next);
+#pragma unroll
+            for (int c = 0; c < C / 32; ++c)
+                o[c] *= by;
+            value_base = next;
+            stage(k0, apart, std::integral_constant<int, kBF16> {});
+        }
+        else
+            stage(k0, apart, std::integral_constant<int, OT> {});
         const int bad = bad_pages(k0); // (the next tile's take their place)
-        const float known = ST == kE4M3 ? ldexpf(unit, key_base - kExponentBias) : unit;
+        // (Held below infinity: a score of zero stays zero.)
+        const float known = ldexpf(1.f, min(key_base - kExponentBias - shift, 127));
         lds_barrier();
         if (k0 + kChunkKeys < end)
             load(k0 + kChunkKeys);
@@ -457,17 +460,16 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FU
             __builtin_amdgcn_s_setprio(0);
             // Value 4i + r of s is key 8i + 4h + r of the 32. Scores in powers of two, but
             // for `scale`, which the multiply-add before the powers takes in.
-            float scale = ST == kE4M3 ? known : unit;
+            float scale = known;
             if (ST == kE4M3 && apart)
             {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                 {
-                    const float4v kp = *reinterpret_cast<const float4v*>(&key_power[32 * b + 8 * i + 4 * h]);
-                    const float4v vp = *reinterpret_cast<const float4v*>(&value_power[32 * b + 8 * i + 4 * h]);
+                    const int4v powers = *reinterpret_cast<const int4v*>(&key_power[32 * b + 8 * i + 4 * h]);
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        s[4 * i + r] = __builtin_fmaf(s[4 * i + r], known * kp[r], vp[r]);
+                        s[4 * i + r] = ldexpf(s[4 * i + r], powers[r] - shift);
                 }
                 scale = 1.f;
             }
@@ -498,73 +500,77 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FU
                     o[c] *= alpha;
                 m = m_new;
             }
+            u32x4 first_parts[2]; // of the weights
+            auto add_rows = [&](auto type) __attribute__((always_inline)) {
+                constexpr int VT = decltype(type)::value;
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale, -base));
-            float own[4] = {0.f, 0.f, 0.f, 0.f};
-            if (ST == kE4M3 && apart)
-            {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                {
-                    const float4v inverse = *reinterpret_cast<const float4v*>(&value_inverse[32 * b + 8 * i + 4 * h]);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        own[r] += s[4 * i + r] * inverse[r];
-                }
-            }
-            else
+                for (int i = 0; i < 16; ++i)
+                    s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale, -base));
+                float own[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     own[i % 4] += s[i];
-            l += (own[0] + own[1]) + (own[2] + own[3]);
-            u32x4 weights[2][kParts];
+                l += (own[0] + own[1]) + (own[2] + own[3]);
+                u32x4 weights[2][parts_of<VT>()];
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+                for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                    for (int i = 0; i < 4; ++i)
+                    {
+                        uint32_t cut[3];
+                        cut_pair<VT>(s[8 * t + 2 * i], s[8 * t + 2 * i + 1], cut);
+#pragma unroll
+                        for (int p = 0; p < parts_of<VT>(); ++p)
+                            weights[t][p][i] = cut[p];
+                    }
+                __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
                 {
-                    uint32_t cut[3];
-                    cut_pair<OT>(s[8 * t + 2 * i], s[8 * t + 2 * i + 1], cut);
-#pragma unroll
-                    for (int p = 0; p < kParts; ++p)
-                        weights[t][p][i] = cut[p];
-                }
-            __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-            {
-                u32x4 value[C / 32];
-#pragma unroll
-                for (int c = 0; c < C / 32; ++c)
-                    value[c] = vs[value_slot(32 * c + n, 4 * b + 2 * t + h)];
-#pragma unroll
-                for (int p = kParts - 1; p >= 0; --p)
+                    u32x4 value[C / 32];
 #pragma unroll
                     for (int c = 0; c < C / 32; ++c)
-                        o[c] = mfma32<OT>(value[c], weights[t][p], o[c]);
-            }
-            __builtin_amdgcn_s_setprio(0);
+                        value[c] = vs[value_slot(32 * c + n, 4 * b + 2 * t + h)];
+#pragma unroll
+                    for (int p = parts_of<VT>() - 1; p >= 0; --p)
+#pragma unroll
+                        for (int c = 0; c < C / 32; ++c)
+                            o[c] = mfma32<VT>(value[c], weights[t][p], o[c]);
+                    if (ST != kE4M3)
+                        first_parts[t] = weights[t][0];
+                }
+                __builtin_amdgcn_s_setprio(0);
+            };
+            if (ST == kE4M3 && wide)
+                add_rows(std::integral_constant<int, kBF16> {});
+            else
+                add_rows(std::integral_constant<int, OT> {});
             if (odd) // (rare: infinities or NaN among the new rows' values)
             {
                 uint32_t parts[8]; // (opaque: nothing of this is worked out before it is needed)
+                if constexpr (ST != kE4M3)
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                {
-                    parts[i] = weights[i / 4][0][i % 4];
-                    asm("" : "+v"(parts[i]));
-                }
+                    for (int i = 0; i < 8; ++i)
+                    {
+                        parts[i] = first_parts[i / 4][i % 4];
+                        asm("" : "+v"(parts[i]));
+                    }
 #pragma unroll 1
                 for (int key = 0; key < 32; ++key)
                 {
                     // Key 16t + 8i + 4h + r is value 4i + r of lane half h's weights t. (Only
-                    // that a weight is not zero matters: the first part of it does.)
-                    uint32_t held = 0;
+                    // that a weight is not zero matters: the first part of it does. E4M3 has no
+                    // infinities, and NaN is NaN by any weight.)
+                    float weight = 1.f;
+                    if constexpr (ST != kE4M3)
+                    {
+                        uint32_t held = 0;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (8 * (key / 16) + 4 * (key / 8 % 2) + key % 4 == i)
-                            held = i % 2 == 0 ? parts[i / 2] << 16 : parts[i / 2] & 0xFFFF0000u;
-                    const float weight = __uint_as_float(__shfl(held, n + 32 * (key / 4 % 2)));
+                        for (int i = 0; i < 16; ++i)
+                            if (8 * (key / 16) + 4 * (key / 8 % 2) + key % 4 == i)
+                                held = i % 2 == 0 ? parts[i / 2] << 16 : parts[i / 2] & 0xFFFF0000u;
+                        weight = __uint_as_float(__shfl(held, n + 32 * (key / 4 % 2)));
+                    }
                     const int position = from + key;
                     const int page = page_of(table, rows.table_width, cache.page_shift, cache.pages, position);
                     if (position >= seen || page < 0)
@@ -587,12 +593,12 @@ __global__ void __launch_bounds__(kChunkWaves* kWave, (kChunkOccupancy<ST, C, FU
     }
 
     // o[c][4i + r] is channel 32c + 8i + 4h + r of pair n; times the values' power.
-    l = halves_sum(l);
+    l = halves_sum(l) * (ST == kE4M3 ? ldexpf(1.f, -kSumShift) : 1.f);
     if (tl.poisoned)
         l = __builtin_nanf("");
     if (!real)
         return;
-    const float power = ldexpf(1.f, value_base - kExponentBias);
+    const float power = ST == kE4M3 ? ldexpf(1.f, value_base - kExponentBias - kSumShift) : 1.f;
     const float by = used > 1 ? power : l == 0.f ? 0.f : power / l;
     const int unit_index = ((int) blockIdx.z * (int) gridDim.y + (int) blockIdx.y) * cache.heads + head;
     float* const part = partial_row(split, unit_index, which, pair - tl.first, width);
