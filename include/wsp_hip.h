@@ -212,7 +212,8 @@ typedef struct wsp_paged_rows
 {
     int sequences;
     int rows;            /* rows the packed tensors hold, at least starts[sequences] */
-    int max_count;       /* attention: no sequence has more new rows (more are left as they were) */
+    int max_count;       /* attention: no sequence has more new rows (more are left as they were); as many
+                            times the query heads a cached one serves, 3·2^29 at most */
     int max_length;      /* attention: no length is larger, nor than 2^30 (else that sequence's rows are NaN) */
     int table_width;     /* pages a row of the table names */
     const int* starts;   /* device [sequences + 1] */

@@ -33,3 +33,10 @@ def test_the_joins_cases_are_cut_as_they_say(plan):
     for given in joins.CUT_ROWS:
         tile_rows, splits, _, fused = plan(*given[1:], joins.PAGE)
         assert tile_rows < 128 and splits == given[0] and fused == (splits <= 16), given
+
+
+def test_the_largest_calls_are_counted_or_refused():
+    subprocess.run(["make", "-s", "_build/paged_extents_check"], cwd=NATIVE, check=True)
+    result = subprocess.run([os.path.join(NATIVE, "_build", "paged_extents_check")], capture_output=True, text=True,
+                            timeout=60)
+    assert result.returncode == 0 and "FAIL" not in result.stdout, result.stdout + result.stderr

@@ -101,9 +101,8 @@ int wsp_hip_paged_attention(wsp_hip_ctx* ctx, const wsp_paged_cache* cache, cons
         return WSP_ERR_ARGUMENT;
     char why[256];
     int status = wsp::paged::refusal(cache, rows, why, sizeof(why));
-    if (status == WSP_OK && (heads <= 0 || heads % cache->heads != 0))
-        status = wsp::paged::say(why, sizeof(why), WSP_ERR_SHAPE, "paged attention: %d query heads over %d cached ones",
-                                 heads, cache->heads);
+    if (status == WSP_OK)
+        status = wsp::paged::refusal_of_attention(cache, rows, heads, why, sizeof(why));
     if (status == WSP_OK)
         status = wsp::paged::refusal_of_tensor(cache, rows, "query", q, heads, q_stride, why, sizeof(why));
     if (status == WSP_OK)

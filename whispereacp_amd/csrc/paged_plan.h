@@ -226,4 +226,20 @@ inline int refusal_of_tensor(const wsp_paged_cache* cache, const wsp_paged_rows*
                    cache->head_width, stride);
     return WSP_OK;
 }
+
+// The same for the query heads of an attention call. The kernels count a sequence's
+// pairs (new row, query head of a cached head's group) in 32 bits, a tile past the last.
+constexpr int kMostPairs = (1 << 30) + (1 << 29);
+
+inline int refusal_of_attention(const wsp_paged_cache* cache, const wsp_paged_rows* rows, int heads, char* why,
+                                size_t size)
+{
+    if (heads <= 0 || heads % cache->heads != 0)
+        return say(why, size, WSP_ERR_SHAPE, "paged attention: %d query heads over %d cached ones", heads, cache->heads);
+    const int count = std::min(rows->rows, rows->max_count), group = heads / cache->heads;
+    if ((long long) count * group > kMostPairs)
+        return say(why, size, WSP_ERR_CAPACITY, "paged attention: %d rows of a sequence times %d query heads a cached one",
+                   count, group);
+    return WSP_OK;
+}
 } // namespace wsp::paged
