@@ -70,7 +70,8 @@ typedef struct wsp_hip_ctx wsp_hip_ctx;
  * default stream) and sizes its workspaces for `shape` (attention partials,
  * argmax candidates, and the 16-bit parts of a product's rows: six bytes for
  * each value of the longest input over the widest layer, 46 MB at large-v3 and
- * 16 MB at least; 64 MB for the paged attention's partial rows). Replaces
+ * 16 MB at least; the paged attention's partial rows share them, 64 MB at
+ * least here, the products' size alone in a Net's context). Replaces
  * KernelNet::prepare's scratch and the SingleQueryAttention/Argmax prepare()
  * sizing (Net/KernelNet.cpp:133-207, Kernels/SingleQueryAttention.cpp:32-60,
  * Kernels/Argmax.cpp:26-40). */

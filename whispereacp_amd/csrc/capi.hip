@@ -51,11 +51,8 @@ int context_hip(Context* ctx, hipError_t e, const char* what)
 {
     return hip_status(ctx, e, what);
 }
-} // namespace wsp
 
-extern "C" {
-
-int wsp_hip_ctx_create(const wsp_decoder_shape* shape, int device, void* stream, wsp_hip_ctx** out)
+int context_create(const wsp_decoder_shape* shape, int device, void* stream, size_t least_scratch, Context** out)
 {
     if (shape == nullptr || out == nullptr)
         return WSP_ERR_ARGUMENT;
@@ -74,34 +71,34 @@ int wsp_hip_ctx_create(const wsp_decoder_shape* shape, int device, void* stream,
 
     int status = hip_status(ctx, hipSetDevice(device), "hipSetDevice");
     if (status == WSP_OK)
-        status = hip_status(ctx, wsp::ops::prepare_split_products(), "products");
+        status = hip_status(ctx, ops::prepare_split_products(), "products");
     if (status == WSP_OK)
     {
         const int head_width = shape->width / shape->heads;
         const int longest = std::max(shape->max_positions, shape->cross_positions);
         size_t floats = 0;
         for (int q = 1; q <= shape->max_positions; ++q)
-            floats = std::max(floats, wsp::ops::attention_workspace_floats(shape->heads, q, longest,
+            floats = std::max(floats, ops::attention_workspace_floats(shape->heads, q, longest,
                                                                            head_width));
         ctx->attention_floats = std::max<size_t>(floats, 1);
         ctx->argmax_candidates =
-            (size_t) shape->max_positions * wsp::ops::argmax_groups(shape->vocabulary_size);
+            (size_t) shape->max_positions * ops::argmax_groups(shape->vocabulary_size);
         // Every product over a window's rows in one piece (46 MB at large-v3);
         // longer ones go in slabs, of no less than 16 MB (546 rows of 5120 as
         // three parts).
         ctx->parts_bytes = std::max<size_t>(
-            16 << 20, wsp::ops::parts_bytes((size_t) longest * std::max(shape->width, shape->feed_forward_width)));
+            16 << 20, ops::parts_bytes((size_t) longest * std::max(shape->width, shape->feed_forward_width)));
         // One block: the attention workspace, the argmax candidates, the paged
-        // attention's counters, the parts, the paged attention's partial rows.
+        // attention's counters, the parts, which the paged attention's partial rows
+        // share (nothing of either outlives a call).
         auto rounded = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
-        const size_t attention = rounded(std::max(ctx->attention_floats, wsp::ops::kQueryAttentionFloats)
+        const size_t attention = rounded(std::max(ctx->attention_floats, ops::kQueryAttentionFloats)
                                          * sizeof(float));
         const size_t candidates = rounded(ctx->argmax_candidates * sizeof(float));
-        const size_t counters = rounded(wsp::paged::kSplitUnits * sizeof(unsigned int));
+        const size_t counters = rounded(paged::kSplitUnits * sizeof(unsigned int));
+        ctx->paged_bytes = std::max(ctx->parts_bytes, least_scratch);
         char* block = nullptr;
-        status = hip_status(ctx, hipMalloc(&block, attention + 2 * candidates + counters
-                                                       + rounded(ctx->parts_bytes) + wsp::paged::kPartialBytes),
-                            "workspace");
+        status = hip_status(ctx, hipMalloc(&block, attention + 2 * candidates + counters + ctx->paged_bytes), "workspace");
         if (status == WSP_OK)
         {
             ctx->attention_workspace = reinterpret_cast<float*>(block);
@@ -109,18 +106,17 @@ int wsp_hip_ctx_create(const wsp_decoder_shape* shape, int device, void* stream,
             ctx->argmax_indices = reinterpret_cast<uint32_t*>(block + attention + candidates);
             ctx->paged_counters = reinterpret_cast<unsigned int*>(block + attention + 2 * candidates);
             ctx->parts = block + attention + 2 * candidates + counters;
-            ctx->paged_partials = block + attention + 2 * candidates + counters + rounded(ctx->parts_bytes);
             // The prompt attention's per-head counters start at zero (each launch
             // leaves them zero again).
             status = hip_status(ctx, hipMemset(ctx->attention_workspace, 0,
-                                               wsp::ops::kAttentionCounters * sizeof(unsigned int)),
+                                               ops::kAttentionCounters * sizeof(unsigned int)),
                                 "attention workspace");
             if (status == WSP_OK) // (the same of the paged attention's)
                 status = hip_status(ctx, hipMemset(ctx->paged_counters, 0, counters), "paged attention");
         }
     }
     if (status == WSP_OK)
-        status = wsp::fused_prepare(ctx);
+        status = fused_prepare(ctx);
     if (status != WSP_OK)
     {
         wsp_hip_ctx_destroy(ctx);
@@ -128,6 +124,14 @@ int wsp_hip_ctx_create(const wsp_decoder_shape* shape, int device, void* stream,
     }
     *out = ctx;
     return WSP_OK;
+}
+} // namespace wsp
+
+extern "C" {
+
+int wsp_hip_ctx_create(const wsp_decoder_shape* shape, int device, void* stream, wsp_hip_ctx** out)
+{
+    return wsp::context_create(shape, device, stream, wsp::paged::kPartialBytes, out);
 }
 
 void wsp_hip_ctx_destroy(wsp_hip_ctx* ctx)

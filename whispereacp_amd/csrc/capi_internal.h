@@ -26,9 +26,10 @@ struct wsp_hip_ctx
     void* parts = nullptr;
     size_t parts_bytes = 0;
 
-    // The paged attention's partial rows (paged::kPartialBytes), and its counters
-    // (paged::kSplitUnits, zero between calls).
-    void* paged_partials = nullptr;
+    // The paged attention's partial rows lie where the parts do, with more room behind
+    // them in a context of wsp_hip_ctx_create; its counters (paged::kSplitUnits) are
+    // zero between calls.
+    size_t paged_bytes = 0;
     unsigned int* paged_counters = nullptr;
 
     void* fused = nullptr; // fused-step state (fused_step.hip)
@@ -44,6 +45,10 @@ struct wsp_hip_ctx
 namespace wsp
 {
 using Context = wsp_hip_ctx;
+
+// wsp_hip_ctx_create with a scratch of at least `least_scratch` bytes: the nets' own
+// contexts ask for none beyond their products'.
+int context_create(const wsp_decoder_shape* shape, int device, void* stream, size_t least_scratch, Context** out);
 
 int context_fail(Context* ctx, int code, const char* message);
 int context_hip(Context* ctx, hipError_t e, const char* what);

@@ -1,6 +1,7 @@
 // Argmax (Kernels/Argmax.cpp:17-81): a context sized for the rows and the row
 // length once, then the two-stage masked argmax per encode().
 #include "../../../include/whispereacp/Argmax.h"
+#include "../capi_internal.h"
 #include "host_common.h"
 
 #include <stdexcept>
@@ -21,7 +22,7 @@ void Argmax::prepare(const Device& device, int rowCount, int rowLength, void* hi
     ctx = nullptr;
     // A context whose argmax workspace covers rowCount rows of rowLength.
     const wsp_decoder_shape shape {4, 1, 1, 4, rowLength, rowCount, 1};
-    const int status = wsp_hip_ctx_create(&shape, device.index, hipStream, &ctx);
+    const int status = wsp::context_create(&shape, device.index, hipStream, 0, &ctx);
     if (status != WSP_OK)
         throwForStatus(status, "Argmax::prepare: the kernel context could not be created");
     rowCapacity = rowCount;

@@ -3,6 +3,7 @@
 // scratch buffers shared by liveness) and then issues the instructions in
 // order, each one or two C-ABI calls on the context's stream.
 #include "../../../include/whispereacp/HipNet.h"
+#include "../capi_internal.h"
 #include "host_common.h"
 
 #include <array>
@@ -56,7 +57,7 @@ void HipNet::prepare(const Device& deviceToUse, const HipNetLayout& layout, void
     wsp_hip_ctx_destroy(ctx);
     ctx = nullptr;
     const wsp_decoder_shape shape = layout.shape.toC();
-    const int status = wsp_hip_ctx_create(&shape, device.index, hipStream, &ctx);
+    const int status = wsp::context_create(&shape, device.index, hipStream, 0, &ctx);
     if (status != WSP_OK)
         throwForStatus(status, "HipNet::prepare: the kernel context could not be created");
 

@@ -111,7 +111,7 @@ int wsp_hip_paged_attention(wsp_hip_ctx* ctx, const wsp_paged_cache* cache, cons
         return refused(ctx, status, why);
     return run(ctx, rows, "paged attention", [&] {
         return wsp::paged::attention(ctx->stream, *cache, *rows, q, q_stride, heads, causal != 0, scale, out,
-                                     out_stride, {ctx->paged_partials, wsp::paged::kPartialBytes, ctx->paged_counters});
+                                     out_stride, {ctx->parts, ctx->paged_bytes, ctx->paged_counters});
     });
 }
 

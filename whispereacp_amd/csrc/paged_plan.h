@@ -119,7 +119,7 @@ constexpr int kJoinRows = 4096;   // partial rows that one block joins
 // and 23.5).
 constexpr int kFusedSplits = 16;
 constexpr int kMostSequences = 65535; // a launch's z extent
-constexpr size_t kPartialBytes = (size_t) 64 << 20; // a context's room for partial rows
+constexpr size_t kPartialBytes = (size_t) 64 << 20; // of wsp_hip_ctx_create's contexts, for partial rows
 
 inline Plan plan_attention(const wsp_paged_cache& cache, const wsp_paged_rows& rows, int group, size_t scratch_floats)
 {
