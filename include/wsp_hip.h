@@ -240,8 +240,10 @@ int wsp_hip_paged_read(wsp_hip_ctx* ctx, const wsp_paged_cache* cache, const wsp
  * heads; query head h reads cache head h / (heads / cache heads). scale
  * multiplies the summed dot product. A row that sees no key gets zeros; keys and
  * values that a row does not see do not reach it, whatever they hold. (A row that
- * sees an infinity or NaN in a key is NaN, in F32 storage as fp32 has it; in a
- * value, not finite in that channel.) */
+ * sees a NaN in a key is NaN. An infinity there makes a score of +inf, and the row
+ * NaN, or of -inf, which weighs nothing; in 16-bit storage a query goes in parts,
+ * and NaN may stand for -inf. Rows whose every score is -inf get zeros. A row that
+ * sees an infinity or NaN in a value is not finite in that channel.) */
 int wsp_hip_paged_attention(wsp_hip_ctx* ctx, const wsp_paged_cache* cache, const wsp_paged_rows* rows,
                             const float* q, int q_stride, int heads, int causal, float scale, float* out,
                             int out_stride);

@@ -178,3 +178,44 @@ def test_a_bad_page_beside_rows_of_far_powers(ctx):  # noqa: F811
     got = attend(ctx, case)
     assert np.isnan(got[112 - 70:]).all()
     assert np.array_equal(got[:112 - 70], clean[:112 - 70])
+
+
+@pytest.mark.parametrize("storage", ["F16", "BF16"])
+@pytest.mark.parametrize("count,kv", [(1, 2), (40, 2), (70, 192)])
+def test_infinite_keys_of_16_bits(ctx, storage, count, kv):  # noqa: F811
+    # Rows that see the key: NaN where fp32's score is +inf; where it is -inf, NaN or the row without it.
+    for sign in (1.0, -1.0):
+        case = Case(storage, [count], [120], kv, 1, 64, 16, seed=229)
+        clean = check(ctx, case)
+        seat = 120 - (count + 1) // 2
+        at = (case.table[0, seat // 16], slice(None), seat % 16)
+        case.key_rows[at + (5,)] = sign * np.inf
+        case.quantise()
+        got = attend(ctx, case)
+        first = seat - (120 - count)
+        assert np.array_equal(got[:first], clean[:first])
+        assert first < count
+        case.key_rows[at] = 0
+        case.key_rows[at + (5,)] = sign * 1e4
+        case.q[:, 5::64] += np.where(case.q[:, 5::64] < 0, -1, 1)  # (no query next to zero)
+        case.quantise()
+        without, bound = case.expected(True, np.full(got.shape, 7.25))
+        case.key_rows[at + (5,)] = sign * np.inf
+        case.quantise()
+        got = attend(ctx, case).reshape(count, kv, 64)
+        up = case.q[:, 5::64] * sign > 0
+        assert np.isnan(got[first:][up[first:]]).all()
+        down = got[first:][~up[first:]]
+        near = np.abs(got - without.reshape(got.shape)) <= bound.reshape(got.shape)
+        assert np.all(np.isnan(down) | near[first:][~up[first:]])
+
+
+@pytest.mark.parametrize("count,kv", [(1, 2), (40, 2)])
+def test_rows_whose_every_score_is_minus_infinity(ctx, count, kv):  # noqa: F811
+    # In fp32 storage: no weight at all, through several waves and splits.
+    for length in (120, 1500):
+        case = Case("F32", [count], [length], kv, 1, 64, 16, seed=233)
+        case.q[:, ::64] = 1.0
+        case.key_rows[..., 0] = -np.inf
+        case.quantise()
+        assert np.all(attend(ctx, case) == 0)
