@@ -8,6 +8,7 @@ import subprocess
 import pytest
 
 import test_gpu_paged_joins as joins
+import test_gpu_paged_uses as uses
 
 NATIVE = os.path.join(os.path.dirname(os.path.abspath(__file__)), "native")
 STORAGES = {"F32": 0, "F16": 1, "BF16": 2, "E4M3": 3}
@@ -33,6 +34,16 @@ def test_the_joins_cases_are_cut_as_they_say(plan):
     for given in joins.CUT_ROWS:
         tile_rows, splits, _, fused = plan(*given[1:], joins.PAGE)
         assert tile_rows < 128 and splits == given[0] and fused == (splits <= 16), given
+
+
+def test_the_captured_cases_take_every_kernel_and_join(plan):
+    cuts = {}
+    for name, (storage, counts, longest, kv, group, width, page, _) in uses.CAPTURED.items():
+        tile_rows, splits, _, fused = plan(storage, counts, [longest] * len(counts), kv, group, width, page)
+        cuts[name] = (tile_rows == 128, splits > 1, splits > 16, bool(fused))
+    assert cuts == {"one-span": (False, False, False, True), "joined-in-place": (False, True, False, True),
+                    "joined-after": (False, True, True, False), "fp32": (False, True, False, True),
+                    "chunks": (True, False, False, False), "cut-chunks": (True, True, False, False)}
 
 
 def test_the_largest_calls_are_counted_or_refused():
