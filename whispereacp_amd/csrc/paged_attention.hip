@@ -55,9 +55,10 @@ __device__ __forceinline__ float groups_sum(float v)
 // next 32 keys and values in flight while it works on these. One token over 131072
 // bf16 positions of eight heads of 128, four query heads each: 96 us and 8 of the join,
 // 5.6 TB/s; 64 such sequences of up to 8192 in E4M3 150 us, 4.0 TB/s, where the vector
-// units are busy half the time (16 pairs' softmax for four real ones, and the widening)
+// units are busy two fifths of the time (16 pairs' softmax for four real ones, and the widening)
 // and two waves a SIMD do not hide the rest (a third spills; a second tile in flight,
-// or loads into registers just used up, change nothing). Short sequences are bound by a
+// or loads into registers just used up, change nothing); a row of zeros in every 64
+// positions, which sends their tiles through bf16, 166 us. Short sequences are bound by a
 // block's chain start, page, keys, scores, values, merge: 5.6 us for one stream of 131
 // positions, 11 for 32 of up to 448 in 20 heads. fp32 is bound by its matrix
 // instructions: five rows over up to 1500 positions of 16 heads of 80, eight streams,
@@ -109,8 +110,9 @@ __device__ __forceinline__ void load_tile(const Cache& cache, const Pages& pages
         const size_t row = pool_row(max(page, 0), head, (second ? k0 + 16 : k0) & mask, cache.heads, cache.page_shift);
         if constexpr (ST == kE4M3) // (looked at first)
         {
-            t.ke[b] = *(const __attribute__((address_space(1))) u32u*) (cache.key_exponents + row + (uint32_t) (4 * g));
-            t.ve[b] = *(const __attribute__((address_space(1))) u32u*) (cache.value_exponents + row + (uint32_t) (4 * g));
+            using Four = const __attribute__((address_space(1))) u32u;
+            t.ke[b] = *(Four*) (cache.key_exponents + row + (uint32_t) (4 * g));
+            t.ve[b] = *(Four*) (cache.value_exponents + row + (uint32_t) (4 * g));
         }
         const char* keys = static_cast<const char*>(cache.keys) + row * row_bytes;
         const char* values = static_cast<const char*>(cache.values) + row * row_bytes;

@@ -63,10 +63,10 @@ __device__ __forceinline__ void lds_barrier()
 // While a tile is worked on the next is in flight to registers, and two blocks a CU
 // fill each other's barriers; a wave at the matrix cores goes before one at vector
 // work. Bound by both together: two chunks of 2048 rows over 16384 E4M3 positions (32
-// query heads over eight, heads of 128) take 2.0 to 2.2 ms, 0.5 PFLOP/s of the
-// algorithm and twice that in two-part products, of the 1.08 an 8192-cubed fp16 library
-// product reaches; the matrix cores are busy 44% of the time, the vector units 47%,
-// seldom at once. (Eight waves a block, each over half the keys: 2.6 ms, with two tiles
+// query heads over eight, heads of 128) take 2.1 ms, 0.5 PFLOP/s of the algorithm and twice
+// that in two-part products, of the 1.08 an 8192-cubed fp16 library product reaches; the
+// matrix cores are busy 43% of the time, the vector units 45%, seldom at once (with a
+// value row of zeros in every 64 positions 2.55 ms). (Eight waves a block, each over half the keys: 2.6 ms, with two tiles
 // in LDS 3.6, its spills waiting for the loads in flight.) The accumulators are the
 // matrix cores' own through all keys: 1.2·10^-6 off in that case, 4·10^-7 where every 32
 // keys are summed apart, at 32 more vector instructions a tile.

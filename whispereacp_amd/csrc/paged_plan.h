@@ -102,10 +102,13 @@ struct Plan
 
 constexpr int kChunkRows = 128;   // of the kernel for many rows
 constexpr int kChunkBlocks = 384; // from so many of its blocks on it is taken
-// Least keys of a cut of its (4096 pairs over 30000 keys of 8 heads of 64: 980 us
-// uncut, 724 in three).
+// Least keys of a cut of its (4096 pairs over 30000 E4M3 keys of 8 heads of 64: 1016 us
+// uncut, 676 in three; of 128, 1652 and 1205).
 constexpr int kChunkSpan = 2048;
-constexpr int kRoundBlocks = 768; // blocks that run at once, three a CU
+// Blocks that run at once, three a CU: of 16 and 32 rows, and of 128 rows of 64-wide fp16 and
+// E4M3 heads. (The others of 128 rows run two a CU or one, so their cuts may take more than
+// a round: 4096 pairs over 30000 bf16 keys of 8 heads of 128, 1726 us in three, 2172 uncut.)
+constexpr int kRoundBlocks = 768;
 constexpr int kLeastSpan = 256;   // two turns of a block's waves
 // Longer spans are cut even where the blocks already fill the chip: lengths differ. (64
 // sequences of up to 8192, eight cached heads of 128 in E4M3: 189 us in spans of 1024,
@@ -143,8 +146,10 @@ inline Plan plan_attention(const wsp_paged_cache& cache, const wsp_paged_rows& r
     const long long filled =
         ((long long) rows.rows * group / kChunkRows + rows.sequences / 2 + 1) * heads; // about
     long long chunk_splits = kRoundBlocks / chunks;
-    if (chunks < kRoundBlocks / 3 && chunk_splits < keys / kMostSpan) // (four sequences of up to 54000
-        chunk_splits = keys / kMostSpan;                              // keys: 489 us in 7, 363 in 13)
+    // (Lengths differ: 200 rows of each of four sequences of up to 54000 fp16 keys of 13 heads of
+    // 64, 419 us in 7 cuts and 325 in 13; all four of 54000, 478 and 503.)
+    if (chunks < kRoundBlocks / 3 && chunk_splits < keys / kMostSpan)
+        chunk_splits = keys / kMostSpan;
     if (chunk_splits > kFusedSplits)
         chunk_splits = kFusedSplits;
     if (chunk_splits > keys / kChunkSpan)
@@ -235,11 +240,12 @@ inline int refusal_of_attention(const wsp_paged_cache* cache, const wsp_paged_ro
                                 size_t size)
 {
     if (heads <= 0 || heads % cache->heads != 0)
-        return say(why, size, WSP_ERR_SHAPE, "paged attention: %d query heads over %d cached ones", heads, cache->heads);
+        return say(why, size, WSP_ERR_SHAPE, "paged attention: %d query heads over %d cached ones", heads,
+                   cache->heads);
     const int count = std::min(rows->rows, rows->max_count), group = heads / cache->heads;
     if ((long long) count * group > kMostPairs)
-        return say(why, size, WSP_ERR_CAPACITY, "paged attention: %d rows of a sequence times %d query heads a cached one",
-                   count, group);
+        return say(why, size, WSP_ERR_CAPACITY,
+                   "paged attention: %d rows of a sequence times %d query heads a cached one", count, group);
     return WSP_OK;
 }
 } // namespace wsp::paged
