@@ -180,6 +180,27 @@ def test_a_bad_page_beside_rows_of_far_powers(ctx):  # noqa: F811
     assert np.array_equal(got[:112 - 70], clean[:112 - 70])
 
 
+@pytest.mark.parametrize("shape", ["few", "chunks"])
+def test_a_nan_value_beside_rows_of_far_powers(ctx, shape):  # noqa: F811
+    # Rows that see it are not finite in its channel, and as they were in the others;
+    # rows before it are as they were, bit for bit.
+    case = powered(shape, "zeros and 2^70 in turn")
+    case.quantise()
+    clean = check(ctx, case)
+    count, length = case.counts[0], case.lengths[0]
+    row = count // 2
+    position = length - count + row | 1  # (one of those of 2^70)
+    row = position - (length - count)
+    page, place = case.table[0, position // 64], position % 64
+    case.values[page, :, place, 5] = 127
+    got = attend(ctx, case)
+    assert np.array_equal(got[:row], clean[:row]) and np.array_equal(got[count:], clean[count:])
+    hit = got[row:count].reshape(count - row, -1, case.width)
+    assert not np.isfinite(hit[:, :, 5]).any()
+    kept = clean[row:count].reshape(hit.shape)
+    assert np.array_equal(np.delete(hit, 5, 2), np.delete(kept, 5, 2))
+
+
 @pytest.mark.parametrize("storage", ["F16", "BF16"])
 @pytest.mark.parametrize("count,kv", [(1, 2), (40, 2), (70, 192)])
 def test_infinite_keys_of_16_bits(ctx, storage, count, kv):  # noqa: F811
