@@ -102,12 +102,13 @@ struct Plan
 
 constexpr int kChunkRows = 128;   // of the kernel for many rows
 constexpr int kChunkBlocks = 384; // from so many of its blocks on it is taken
-// Least keys of a cut of its (4096 pairs over 30000 E4M3 keys of 8 heads of 64: 1016 us
-// uncut, 676 in three; of 128, 1652 and 1205).
+// Least keys of a cut of its (4096 pairs over 30000 E4M3 keys of 8 heads of 64: 1317 us
+// uncut, 660 in three, 1016 in blocks of 32 rows; of 128, 1617, 1178 and 1652).
 constexpr int kChunkSpan = 2048;
 // Blocks that run at once, three a CU: of 16 and 32 rows, and of 128 rows of 64-wide fp16 and
 // E4M3 heads. (The others of 128 rows run two a CU or one, so their cuts may take more than
-// a round: 4096 pairs over 30000 bf16 keys of 8 heads of 128, 1726 us in three, 2172 uncut.)
+// a round: 4096 pairs over 30000 bf16 keys of 8 heads of 128, 1725 us in three, 1665 uncut;
+// in fp16, 1074 and 1342.)
 constexpr int kRoundBlocks = 768;
 constexpr int kLeastSpan = 256;   // two turns of a block's waves
 // Longer spans are cut even where the blocks already fill the chip: lengths differ. (64
